@@ -81,7 +81,8 @@ int qi_b200_abi_version(void);
 const char* qi_b200_error_string(int code);
 
 /* Device status word of the current device: out4[0] = error (0 none, 1 a
- * bounded wait timed out), out4[1] = kernel tag, out4[2] = wait site,
+ * bounded wait timed out, 2 an index read from device memory was out of its
+ * range), out4[1] = kernel tag, out4[2] = wait site or check,
  * out4[3] = block index.  Synchronous (reads device memory); not for use
  * inside stream capture.  clear != 0 resets it. */
 int qi_b200_device_status(unsigned int* out4, int clear);
@@ -250,6 +251,90 @@ int qi_b200_rms_rope_partials(const void* in0, const void* in1, long long ld_in,
 int qi_b200_attention_short(const void* q, long long ldq, const void* k, long long ldk, const void* vt,
                             long long ldvt, void* o, long long ldo, int sq, int sk, int heads, int head_dim,
                             float scale, cudaStream_t stream);
+
+/* ---- decoder block ------------------------------------------------------
+ * What a served decoder runs between its quantized linears (no counterpart in
+ * the reference, whose DiT is not autoregressive and calls torch here).  All
+ * activations bf16, row strides (ld*) multiples of 8 elements, pointers
+ * 16-byte aligned.
+ *
+ * Residual addition, RMSNorm and per-row 8-bit quantization in one pass:
+ *   h = bf16(x + y), written to x_out (which may be x); without y, h = x
+ *   v = h * weight / sqrt(mean(h^2) + eps)                       (fp32)
+ *   KIND_INT8: s = max(max|v|/127, 1e-10), q = clamp(rint(v/s), -127, 127)
+ *   KIND_FP8_E4M3: s = max(max|v|/448, 1e-12), q = e4m3_rn(v/s), saturating
+ *   KIND_BF16: no codes (q, scales unused)
+ * xn (optional with codes, required with KIND_BF16) receives bf16(v).
+ * q [M, D] and xn [M, D] are dense; D % 8 == 0, D <= 16384.  A row that holds
+ * an infinity or NaN gets the scale NaN. */
+int qi_b200_rms_norm_quant(int kind, const void* x_bf16, long long ldx, const void* y_bf16, long long ldy,
+                           void* x_out_bf16, long long ld_out, const void* weight_bf16, void* q, float* scales,
+                           void* xn_bf16, int M, int D, float eps, cudaStream_t stream);
+
+/* A paged key-value cache: token t of a sequence lies at place t % page_size
+ * of the page that the sequence's table names at t / page_size.  Strides in
+ * elements; unit stride inside a head; every stride a multiple of 16 bytes.
+ * fp8: E4M3 codes whose values are code * scale (scale[0] for K, scale[1]
+ * for V; one value, or one per key head where scale_per_head is set). */
+typedef struct qi_b200_paged_cache {
+  void* k;
+  void* v;
+  long long page_stride[2], slot_stride[2], head_stride[2]; /* K, V */
+  int pages, page_size;
+  int fp8;
+  const float* scale[2];
+  int scale_per_head[2];
+} qi_b200_paged_cache;
+
+/* Rotary positions with several axes on the q and k columns of a projection.
+ * Pair i of a head (i < pairs) turns by positions[axes_of[i], m] * freqs[i]:
+ *   (x, y) -> (x cos - y sin, x sin + y cos)
+ * of elements (2i, 2i+1) (interleaved) or (i, i + pairs); elements from
+ * 2 * pairs on pass unchanged.  positions [axes, M] int32 or int64
+ * (positions64), freqs [pairs] fp64 radians, axes_of [pairs] int32 in
+ * [0, axes).  The angle is reduced in 64 bits, so far positions keep full
+ * precision.  q [M, heads * head_dim] -> q_out (may be q itself).  Without a
+ * cache: k [M, kv_heads * head_dim] -> k_out (may be k; kv_heads 0: q only).
+ * With a cache: rotated k and unchanged v are written to slot slots[m], and
+ * the rotated k also to k_out unless that is null (a prompt's attention reads
+ * it there).  slots [M] int32 or int64 (slots64): page slots[m] / page_size,
+ * place slots[m] % page_size; a negative slot writes nothing, a slot behind the last page writes nothing
+ * and sets the device status word (code 2).  Two rows must not name the same
+ * slot.  head_dim % 16 == 0, <= 512; pairs % 8 == 0. */
+int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
+                      void* q_out, long long ldq_out, void* k_out, long long ldk_out, const void* positions,
+                      int positions64, const double* freqs, const int* axes_of, int pairs, int axes, int interleaved,
+                      int M, int heads, int kv_heads, int head_dim, const qi_b200_paged_cache* cache,
+                      const void* slots, int slots64, cudaStream_t stream);
+
+/* Attention over packed sequences: rows cu_q[b] .. cu_q[b+1] of q attend the
+ * rows cu_k[b] .. cu_k[b+1] of k and v (cu_* int32 [n_seq + 1], device,
+ * ascending); with causal, query i of a sequence sees the keys
+ * j <= i + (lk - lq).  A query that sees no key gives zeros.  Query head h
+ * reads key head h / (heads / kv_heads).  head_dim 64 or 128.  bf16 in and
+ * out, fp32 scores and sums, probabilities rounded to bf16 before the product
+ * with V.  lse (optional, fp32 [total_q, heads]): log of the sum of
+ * exp(scale q.k), -inf where no key is seen.  Rows of out (and lse) outside
+ * every sequence are left as they were.  Keys and values inside a sequence
+ * have to be finite. */
+int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
+                             void* out, long long ldo, float* lse, const int* cu_q, const int* cu_k, int n_seq,
+                             int total_q, int total_k, int heads, int kv_heads, int head_dim, int causal, float scale,
+                             cudaStream_t stream);
+
+/* Attention of one new token per sequence over a paged cache: row b of q
+ * attends the first lengths[b] tokens (int32, device) of sequence b, whose
+ * pages are page_table[b, :] (int32, device, row stride ld_table, max_pages
+ * columns).  A length of 0 gives zeros (lse -inf).  A page outside the cache
+ * or a length behind the table reads nothing: those keys take no part, and
+ * the device status word is set (code 2).  The workspace holds partial
+ * results of sequences that several SMs share; it needs no initialization and
+ * may be used again by the next call on the stream. */
+int qi_b200_attention_paged_workspace_bytes(int head_dim, size_t* bytes);
+int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_cache* cache, const int* page_table,
+                            long long ld_table, int max_pages, const int* lengths, void* out, long long ldo,
+                            float* lse, int B, int heads, int kv_heads, int head_dim, float scale, void* workspace,
+                            size_t workspace_bytes, cudaStream_t stream);
 
 /* Per-token FP8: s = max(amax/448, 1e-12), q = e4m3_rn(clamp(x/s, +-448)).
  * Generalises backends/flashrt_fp8_ops.py:38-48 (per tensor) to per row. */

@@ -82,8 +82,24 @@ SIGNATURES = {
     "qi_b200_w4a16_linear": [_P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P],
     "qi_b200_quantize_nvfp4": [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P],
     "qi_b200_nvfp4_gemm": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _LL, _I, _I, _I, _I, _P],
+    "qi_b200_rms_norm_quant": [_I, _P, _LL, _P, _LL, _P, _LL, _P, _P, _P, _P, _I, _I, _F, _P],
+    "qi_b200_rope_axes": [_P, _LL, _P, _LL, _P, _LL, _P, _LL, _P, _LL, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I,
+                          _P, _P, _I, _P],
+    "qi_b200_attention_packed": [_P, _LL, _P, _LL, _P, _LL, _P, _LL, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P],
+    "qi_b200_attention_paged_workspace_bytes": [_I, _P],
+    "qi_b200_attention_paged": [_P, _LL, _P, _P, _LL, _I, _P, _P, _LL, _P, _I, _I, _I, _I, _F, _P, ctypes.c_size_t,
+                                _P],
     "qi_b200_nvfp4_linear": [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
 }
+
+
+class PagedCache(ctypes.Structure):
+    """``qi_b200_paged_cache`` of the C ABI."""
+
+    _fields_ = [("k", _P), ("v", _P), ("page_stride", _LL * 2), ("slot_stride", _LL * 2), ("head_stride", _LL * 2),
+                ("pages", _I), ("page_size", _I), ("fp8", _I), ("scale", _P * 2), ("scale_per_head", _I * 2)]
+
+
 _RESTYPES = {"qi_b200_error_string": ctypes.c_char_p}
 
 _lock = threading.Lock()
@@ -159,13 +175,21 @@ def device_status(clear: bool = False) -> tuple[int, int, int, int]:
 
 
 class QiB200DeviceError(RuntimeError):
-    """A kernel of this library gave up a bounded wait (device status word set).
+    """A kernel of this library gave up a bounded wait, or met an index outside
+    its range in device memory (device status word set).
 
-    The kernel returned early, so the outputs of the launch that set the word
-    (and of every launch after it on that device) are incomplete."""
+    After a wait the kernel returned early, so the outputs of the launch that
+    set the word (and of every launch after it on that device) are incomplete;
+    after a bad index (a cache page or slot, a length, a rotary axis) that
+    index was left out and everything else was computed."""
 
     def __init__(self, status: tuple):
         self.status = tuple(status)
+        if status[0] == 2:
+            super().__init__(
+                "qi_b200: an index read from device memory is out of range (kernel tag 0x%x, check %d, block %d); "
+                "what it names was left out" % (status[1], status[2], status[3]))
+            return
         super().__init__(
             "qi_b200: a bounded device wait timed out (kernel tag 0x%x, wait site %d, block %d); outputs of the "
             "launches since the last status check are incomplete" % (status[1], status[2], status[3]))
@@ -173,7 +197,8 @@ class QiB200DeviceError(RuntimeError):
 
 def raise_on_device_error(clear: bool = True) -> None:
     """Read the current device's status word (synchronous: the host waits for
-    the device) and raise ``QiB200DeviceError`` if a bounded wait timed out.
+    the device) and raise ``QiB200DeviceError`` if a bounded wait timed out
+    or an index in device memory was out of range.
     ``clear`` resets the word (and the counters an aborted launch may have
     left) so the context can run again.  Call it at a point where the caller
     synchronizes anyway: after a step, between graph replays, at shutdown."""

@@ -1601,3 +1601,8 @@ extern "C" int qi_b200_attention_short(const void* q, long long ldq, const void*
   if (!(scale > 0.0f)) return QI_B200_EINVAL;
   return launch_attn_short_db(q, ldq, k, ldk, vt, ldvt, o, ldo, sq, sk, heads, scale, stream);
 }
+
+// ---------------------------------------------------------------------------
+// Decoder-block operators
+// ---------------------------------------------------------------------------
+#include "decoder_entries.cuh"

@@ -26,6 +26,7 @@ namespace qib {
 enum DeviceError : unsigned int {
   kDevOk = 0,
   kDevWaitTimeout = 1,
+  kDevBadIndex = 2,  // an index read from device memory (page, slot, length, axis) lies outside its range
 };
 
 __device__ unsigned int g_status[4];

@@ -1,0 +1,701 @@
+"""GPU: the decoder-block operators against plain 64-bit implementations.
+
+Tolerances, from the roundings each kernel makes (half a step relative to the
+value: bf16 2^-8, fp16 2^-11, E4M3 2^-4 of a normal value):
+
+* ``rms_norm_quant``: v / s carries fp32 errors only.  The sum of squares adds
+  at most 64 terms in a row per thread and 10 levels of a tree, so its relative
+  error is below 74 * 2^-24; square root, two divisions and three products add
+  a few 2^-24 more: 2^-17 in all covers it.  A code is then at most half a
+  step plus 2^-17 |v / s| away from the exact v / s.
+* ``rope_axes``: the turn is reduced in 64 bits, cos and sin are off by less
+  than 2^-21 in all, so a rotated element by (|x| + |y|) 2^-20 plus the
+  rounding of the output's type.
+* attention: probabilities round once (bf16 2^-8, fp16 2^-11 in an E4M3
+  cache), the output once (2^-8).  With A = sum_j p_j |v_j| the result is off
+  by at most r_p A + 2^-8 |o|, plus the scores' fp32 errors: (D + 16) 2^-24
+  times the largest scale * sum |q| |k|, twice (numerator and sum), times A.
+  Second-order terms are below 1 % of that.
+"""
+
+import math
+
+import pytest
+import torch
+
+from qi_b200 import _lib, kernels as K
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF = torch.bfloat16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _device():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    _lib.load()
+    torch.cuda.set_device(0)
+    yield
+    torch.cuda.synchronize()
+    st = _lib.device_status(clear=True)
+    assert st[0] == 0, f"device status word: {st}"
+
+
+def gen(seed):
+    return torch.Generator(device="cpu").manual_seed(seed)
+
+
+def randn(g, *shape, mul=1.0):
+    return (torch.randn(*shape, generator=g) * mul).to(BF).to(DEV)
+
+
+def e4m3_value(codes):
+    return codes.view(torch.float8_e4m3fn).double()
+
+
+def e4m3_half_step(v):
+    """Half the distance of E4M3 values around |v| (64 bits)."""
+    return torch.exp2(torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -6))) - 4)
+
+
+# ---------------------------------------------------------------------------
+# rms_norm_quant
+# ---------------------------------------------------------------------------
+
+
+def check_norm(kind, x, w, y, eps, q, s, h, xn=None):
+    hd = h.double()
+    v = hd * w.double() / torch.sqrt(hd.square().mean(1, keepdim=True) + eps)
+    if xn is not None:
+        assert ((xn.double() - v).abs() <= v.abs() * (2.0 ** -8 + 2.0 ** -17)).all()
+    if kind == _lib.KIND_BF16:
+        return
+    top = 127.0 if kind == _lib.KIND_INT8 else 448.0
+    want = (v.abs().amax(1) / top).clamp_min(1e-10 if kind == _lib.KIND_INT8 else 1e-12)
+    assert ((s.double() - want).abs() <= want * 2.0 ** -17).all()
+    t = v / want[:, None]
+    got = q.double() if kind == _lib.KIND_INT8 else e4m3_value(q)
+    half = torch.full_like(t, 0.5) if kind == _lib.KIND_INT8 else e4m3_half_step(t)
+    assert ((got - t).abs() <= half + t.abs() * 2.0 ** -17).all()
+
+
+@pytest.mark.parametrize("kind", [_lib.KIND_INT8, _lib.KIND_FP8_E4M3, _lib.KIND_BF16])
+@pytest.mark.parametrize("M,D,residual", [
+    (1, 4096, True), (1, 8, False), (3, 520, True), (777, 1024, True), (300, 1000, False), (5, 16384, True),
+    (257, 8192, True), (260, 16384, False), (64, 2056, True), (1024, 264, True),
+])
+def test_rms_norm_quant(kind, M, D, residual):
+    g = gen(M * 31 + D)
+    x, w = randn(g, M, D, mul=3.0), randn(g, D)
+    y = randn(g, M, D) if residual else None
+    h = (x.float() + y.float()).to(BF) if residual else x.clone()
+    xn = torch.empty_like(x)
+    x0 = x.clone()
+    x_out = torch.empty_like(x) if residual else None
+    q, s = K.rms_norm_quant(kind, x, w, y, eps=1e-5, x_out=x_out, xn=xn)
+    assert torch.equal(x, x0)
+    if residual:
+        assert torch.equal(x_out, h)
+    check_norm(kind, x, w, y, 1e-5, q, s, h, xn)
+    q2, s2 = K.rms_norm_quant(kind, x, w, y, eps=1e-5, xn=xn if kind == _lib.KIND_BF16 else None)  # in place
+    if residual:
+        assert torch.equal(x, h)
+    if kind != _lib.KIND_BF16:
+        assert torch.equal(q, q2) and torch.equal(s, s2)
+
+
+def test_rms_norm_quant_strided_rows():
+    g = gen(4)
+    M, D = 50, 640
+    wide, yw, ow = randn(g, M, 3 * D), randn(g, M, D + 8), torch.zeros(M + 2, D + 16, dtype=BF, device=DEV)
+    x, y, w = wide[:, D:2 * D], yw[:, 8:], randn(g, D)
+    q, s = K.rms_norm_quant(_lib.KIND_INT8, x, w, y, x_out=ow[1:-1, :D])
+    want = K.rms_norm_quant(_lib.KIND_INT8, x.contiguous(), w, y.contiguous(), x_out=torch.empty(M, D, dtype=BF, device=DEV))
+    assert torch.equal(q, want[0]) and torch.equal(s, want[1])
+    assert torch.equal(ow[1:-1, :D], (x.float() + y.float()).to(BF))
+    assert ow[0].abs().sum() == 0 and ow[-1].abs().sum() == 0 and ow[:, D:].abs().sum() == 0
+
+
+@pytest.mark.parametrize("kind", [_lib.KIND_INT8, _lib.KIND_FP8_E4M3])
+def test_rms_norm_quant_zero_and_non_finite_rows(kind):
+    x = torch.ones(5, 64, dtype=BF, device=DEV)
+    x[1] = 0
+    x[2, 7] = float("inf")
+    x[3, 9] = float("nan")
+    w = torch.full((64,), 2.0, dtype=BF, device=DEV)
+    q, s = K.rms_norm_quant(kind, x, w)
+    assert s[1].item() == pytest.approx(1e-10 if kind == _lib.KIND_INT8 else 1e-12)
+    assert (q[1] == 0).all()
+    assert torch.isnan(s[2]) and torch.isnan(s[3])
+    assert torch.isfinite(s[[0, 4]]).all() and torch.equal(q[0], q[4])
+
+
+# ---------------------------------------------------------------------------
+# rope_axes
+# ---------------------------------------------------------------------------
+
+
+def rotate_ref(x, heads, D, positions, freqs, axes, interleaved):
+    """(rotated fp64 [M, heads, D], |x| + |y| of each element's pair)."""
+    M, P = x.shape[0], freqs.numel()
+    xd = x.double().reshape(M, heads, D)
+    ang = positions.double()[axes.long()].t() * freqs
+    c, s = ang.cos()[:, None], ang.sin()[:, None]
+    out, mag = xd.clone(), torch.zeros_like(xd)
+    ia = torch.arange(P, device=x.device) * (2 if interleaved else 1)
+    ib = ia + (1 if interleaved else P)
+    a, b = xd[..., ia], xd[..., ib]
+    out[..., ia], out[..., ib] = a * c - b * s, a * s + b * c
+    mag[..., ia] = mag[..., ib] = a.abs() + b.abs()
+    return out, mag
+
+
+@pytest.mark.parametrize("M,hq,hk,D,sections,shared,interleaved,idx", [
+    (1, 32, 8, 128, (64,), True, False, torch.int32),
+    (3120, 24, 24, 128, (22, 21, 21), False, True, torch.int64),
+    (77, 5, 1, 64, (10, 11, 11), True, False, torch.int32),
+    (2500, 4, 2, 64, (16,), False, True, torch.int64),      # half of the head rotates
+    (13, 3, 3, 80, (8, 8, 8), True, False, torch.int32),    # 48 of 80 elements
+    (9, 2, 1, 512, (256,), True, True, torch.int32),
+    (6, 1, 2, 16, (8,), True, False, torch.int32),
+])
+def test_rope_axes(M, hq, hk, D, sections, shared, interleaved, idx):
+    g = gen(M + D)
+    qkv = randn(g, M, (hq + 2 * hk) * D)
+    q, k = qkv[:, :hq * D], qkv[:, hq * D:(hq + hk) * D]
+    freqs, axes = K.rope_axes_frequencies(sections, shared=shared, device=DEV)
+    positions = torch.randint(-5, 1 << 20, (len(sections), M), generator=g).to(idx).to(DEV)
+    positions[:, 0] = (1 << 31) - 1  # the farthest position
+    oq, ok = K.rope_axes(q, k, positions, freqs, axes, D, interleaved=interleaved)
+    # the turn of position 2^31 is exact to 2^-53 relative: 2^-24 of a turn
+    for x, o, h in ((q, oq, hq), (k, ok, hk)):
+        want, mag = rotate_ref(x, h, D, positions, freqs, axes, interleaved)
+        assert ((o.double().view(M, h, D) - want).abs() <= mag * 2.0 ** -20 + want.abs() * 2.0 ** -8).all()
+    before = qkv.clone()
+    K.rope_axes(q, k, positions, freqs, axes, D, interleaved=interleaved, out_q=q, out_k=k)  # in place
+    assert torch.equal(q, oq) and torch.equal(k, ok)
+    assert torch.equal(qkv[:, (hq + hk) * D:], before[:, (hq + hk) * D:])
+    only, none = K.rope_axes(before[:, :hq * D], None, positions, freqs, axes, D, interleaved=interleaved)
+    assert none is None and torch.equal(only, oq)
+
+
+def test_rope_axes_matches_the_dit_table():
+    """The repository's 3-axis video table (fp32 cos / sin) gives the same rotation to the table's own fp32 error."""
+    from qi_b200.dit import CFG5, rope_apply, rope_tables
+
+    spec = CFG5.experts[0]
+    g = gen(3)
+    q = randn(g, spec.tokens, 2 * 128)
+    t = torch.arange(spec.tokens, device=DEV, dtype=torch.int32)
+    positions = torch.stack([t // 120, t % 120 // 10, t % 10]).contiguous()
+    freqs, axes = K.rope_axes_frequencies((22, 21, 21), device=DEV)
+    o, _ = K.rope_axes(q, None, positions, freqs, axes, 128)
+    want = rope_apply(q[None], rope_tables(CFG5, spec, DEV), 2)[0]
+    # both round the same value to bf16: at most one step (2 x 2^-8) where fp32 errors straddle a border
+    assert ((o.float() - want.float()).abs() <= want.float().abs() * 2.0 ** -7 + 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "fp8_one_scale"])
+@pytest.mark.parametrize("M,hq,hk,D,page,layout", [
+    (1, 8, 2, 128, 16, "token"), (50, 4, 4, 64, 7, "head"), (333, 6, 1, 128, 64, "joint"), (2400, 2, 2, 128, 1, "token"),
+])
+def test_rope_axes_store(kind, M, hq, hk, D, page, layout):
+    g = gen(M * 3 + D)
+    qkv = randn(g, M, (hq + 2 * hk) * D)
+    q, k, v = qkv[:, :hq * D], qkv[:, hq * D:(hq + hk) * D], qkv[:, (hq + hk) * D:]
+    freqs, axes = K.rope_axes_frequencies((D // 2,), shared=True, device=DEV)
+    positions = torch.randint(0, 5000, (M,), generator=g).to(DEV)
+    pages = -(-M // page) + 2
+    dt = BF if kind == "bf16" else torch.uint8
+    if layout == "token":
+        kc, vc = (torch.full((pages, page, hk, D), 3, dtype=dt, device=DEV) for _ in range(2))
+    elif layout == "head":
+        kc, vc = (torch.full((pages, hk, page, D), 3, dtype=dt, device=DEV).transpose(1, 2) for _ in range(2))
+    else:
+        both = torch.full((pages, 2, page, hk, D), 3, dtype=dt, device=DEV)
+        kc, vc = both[:, 0], both[:, 1]
+    n_scale = 1 if kind == "fp8_one_scale" else hk
+    ks, vs = (None, None) if kind == "bf16" else (0.01 + 0.02 * torch.rand(2, n_scale, generator=g).to(DEV))
+    slots = torch.randperm(pages * page, generator=g)[:M].to(DEV)
+    slots[::5] = -1  # padding rows
+    ok = torch.zeros(M, hk * D, dtype=BF, device=DEV)
+    oq = K.rope_axes_store(q, k, v, positions, freqs, axes, D, kc, vc, slots, interleaved=False, k_scale=ks, v_scale=vs,
+                           out_k=ok)
+    want_q, want_k = K.rope_axes(q, k, positions, freqs, axes, D, interleaved=False)
+    assert torch.equal(oq, want_q) and torch.equal(ok, want_k)
+    kr, mag = rotate_ref(k, hk, D, positions[None], freqs, axes, False)
+    live = slots >= 0
+    at = slots[live].long()
+    for x, m, c, sc in ((kr, mag, kc, ks), (v.double().reshape(M, hk, D), torch.zeros_like(mag), vc, vs)):
+        got = c[at // page, at % page]
+        if kind == "bf16":
+            assert ((got.double() - x[live]).abs() <= m[live] * 2.0 ** -20 + x[live].abs() * 2.0 ** -8).all()
+        else:
+            s = sc.double().expand(hk)[None, :, None]
+            t = (x[live] / s).clamp(-448, 448)
+            tol = e4m3_half_step(t) + m[live] / s * 2.0 ** -19 + t.abs() * 2.0 ** -22
+            assert ((e4m3_value(got.contiguous()) - t).abs() <= tol).all()
+        rest = torch.ones(pages * page, dtype=torch.bool, device=DEV)
+        rest[at] = False
+        r = rest.nonzero()[:, 0]
+        assert (c[r // page, r % page] == 3).all()  # every other slot as it was
+
+
+def test_rope_axes_store_reports_slots_outside_the_cache():
+    g = gen(1)
+    x = randn(g, 4, 3 * 64)
+    freqs, axes = K.rope_axes_frequencies((32,), device=DEV)
+    kc, vc = (torch.zeros(2, 4, 1, 64, dtype=BF, device=DEV) for _ in range(2))
+    slots = torch.tensor([0, 8, 3, 1 << 40], device=DEV)
+    pos = torch.arange(4, device=DEV)
+    K.rope_axes_store(x[:, :64], x[:, 64:128], x[:, 128:], pos, freqs, axes, 64, kc, vc, slots)
+    with pytest.raises(_lib.QiB200DeviceError, match="out of range"):
+        _lib.raise_on_device_error()
+    assert _lib.device_status()[0] == 0
+    assert torch.equal(vc.view(8, 64)[[0, 3]], x[[0, 2], 128:])
+    assert vc.view(8, 64)[[1, 2, 4, 5, 6, 7]].abs().sum() == 0
+    K.rope_axes(x[:, :64], None, pos, freqs, torch.full_like(axes, 1), 64)  # an axis that positions do not have
+    with pytest.raises(_lib.QiB200DeviceError, match="out of range"):
+        _lib.raise_on_device_error()
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+
+def attend_ref(q, k, v, first, scale, r_p):
+    """fp64 attention of q [a, D] on k, v [b, D]: (o, tolerance, lse); ``first``: query i sees keys <= first + i."""
+    a, b = q.shape[0], k.shape[0]
+    if b == 0:
+        z = torch.zeros_like(q, dtype=torch.float64)
+        return z, z, torch.full((a,), -math.inf, dtype=torch.float64, device=q.device)
+    q, k, v = q.double(), k.double(), v.double()
+    s = scale * q @ k.t()
+    if first is not None:
+        i, j = torch.arange(a, device=q.device)[:, None], torch.arange(b, device=q.device)
+        s = s.masked_fill(j > first + i, -math.inf)
+    top = s.amax(1, keepdim=True).clamp_min(-1e300)
+    e = torch.exp(s - top)
+    l = e.sum(1, keepdim=True)
+    p = torch.where(l > 0, e / l.clamp_min(1e-300), 0.0)
+    o, A = p @ v, p @ v.abs()
+    D = q.shape[1]
+    sabs = (scale * (q.abs() @ k.abs().t())).amax(1, keepdim=True)
+    tol = 1.01 * (r_p * A + 2.0 ** -8 * o.abs() + 2 * (D + 16) * 2.0 ** -24 * sabs * A) + 1e-30
+    return o, tol, (top + l.log())[:, 0]
+
+
+def packed_ref(q, k, v, ql, kl, hq, hk, D, causal, scale):
+    o, tol = (torch.zeros(q.shape, dtype=torch.float64, device=DEV) for _ in range(2))
+    lse = torch.zeros(q.shape[0], hq, dtype=torch.float64, device=DEV)
+    i = j = 0
+    for a, b in zip(ql, kl):
+        for h in range(hq):
+            g = h // (hq // hk)
+            c = slice(h * D, (h + 1) * D)
+            o[i:i + a, c], tol[i:i + a, c], lse[i:i + a, h] = attend_ref(
+                q[i:i + a, c], k[j:j + b, g * D:(g + 1) * D], v[j:j + b, g * D:(g + 1) * D],
+                b - a if causal else None, scale, 2.0 ** -8)
+        i, j = i + a, j + b
+    return o, tol, lse
+
+
+def cu(lens):
+    return torch.tensor([0] + list(lens)).cumsum(0).to(torch.int32).to(DEV)
+
+
+def close_lse(got, want):
+    fin = torch.isfinite(want)
+    assert torch.equal(got[~fin].double(), want[~fin])
+    assert ((got.double() - want)[fin].abs() <= 1e-5 * (1 + want[fin].abs())).all()
+
+
+PACKED = [
+    # q lengths, k lengths (None: the same), heads, kv_heads, D, causal
+    ([1], None, 1, 1, 128, True),
+    ([128], None, 2, 1, 128, True),
+    ([129], None, 1, 1, 64, False),
+    ([256], None, 3, 1, 128, True),
+    ([300, 1, 17, 128, 0, 257, 2], None, 4, 2, 128, True),
+    ([300, 1, 17, 128, 0, 257, 2], None, 3, 3, 64, True),
+    ([64, 200], [700, 513], 8, 2, 64, True),        # chunks after a prefix
+    ([64, 200], [700, 513], 6, 2, 128, False),
+    ([300, 5, 130], [100, 0, 129], 2, 2, 128, True),  # queries in front of every key; no keys at all
+    ([300, 5, 130], [100, 0, 129], 2, 1, 64, False),
+    ([1000], None, 24, 8, 128, True),
+    ([1, 1, 1, 1], [1, 129, 1000, 16], 4, 1, 128, True),
+    ([3] * 70, None, 2, 1, 64, True),               # more sequences than a warp has lanes
+    ([40, 700] * 40, None, 2, 2, 128, True),
+]
+
+
+@pytest.mark.parametrize("ql,kl,hq,hk,D,causal", PACKED)
+def test_attention_packed(ql, kl, hq, hk, D, causal):
+    g = gen(sum(ql) + D + hq)
+    kl = kl or ql
+    q, k, v = randn(g, sum(ql), hq * D), randn(g, sum(kl), hk * D), randn(g, sum(kl), hk * D)
+    lse = torch.full((sum(ql), hq), 7.0, device=DEV)
+    o = K.attention_packed(q, k, v, cu(ql), cu(kl), hq, hk, causal=causal, lse=lse)
+    want, tol, wl = packed_ref(q, k, v, ql, kl, hq, hk, D, causal, D ** -0.5)
+    assert ((o.double() - want).abs() <= tol).all(), ((o.double() - want).abs() / tol).max().item()
+    close_lse(lse, wl)
+    assert torch.equal(o, K.attention_packed(q, k, v, cu(ql), cu(kl), hq, hk, causal=causal))
+
+
+@pytest.mark.parametrize("mul,scale", [(8.0, None), (1.0, 3.0), (0.02, 1e-3)])
+def test_attention_packed_growing_maxima(mul, scale):
+    """Large logits, with keys that grow towards the front, so that the running maximum moves in every step."""
+    g = gen(11)
+    n, hq, D = 1500, 2, 128
+    q, v = randn(g, n, hq * D), randn(g, n, hq * D)
+    k = (torch.randn(n, hq * D, generator=g) * torch.linspace(mul, 0.1 * mul, n)[:, None]).to(BF).to(DEV)
+    o = K.attention_packed(q, k, v, cu([n]), cu([n]), hq, hq, scale=scale)
+    want, tol, _ = packed_ref(q, k, v, [n], [n], hq, hq, D, True, scale or D ** -0.5)
+    assert ((o.double() - want).abs() <= tol).all()
+
+
+def test_attention_packed_strided_and_rows_left_alone():
+    """Slices of one fused projection with padding rows behind the last sequence that hold NaN, a neighbour whose
+    values are NaN, and an output whose other rows and columns keep their contents."""
+    g = gen(12)
+    ql, hq, hk, D = [150, 37], 4, 2, 64
+    T = sum(ql)
+    qkv = randn(g, T + 9, (hq + 2 * hk) * D + 8)
+    qkv[T:] = float("nan")
+    q, k, v = qkv[:, :hq * D], qkv[:, hq * D:(hq + hk) * D], qkv[:, (hq + hk) * D:(hq + 2 * hk) * D]
+    big = torch.full((T + 9, hq * D + 16), 5.0, dtype=BF, device=DEV)
+    lse = torch.full((T + 9, hq), 5.0, device=DEV)
+    K.attention_packed(q, k, v, cu(ql), cu(ql), hq, hk, out=big[:, 8:8 + hq * D], lse=lse)
+    want, tol, _ = packed_ref(q[:T], k[:T], v[:T], ql, ql, hq, hk, D, True, D ** -0.5)
+    assert ((big[:T, 8:8 + hq * D].double() - want).abs() <= tol).all()
+    assert (big[T:] == 5).all() and (big[:, :8] == 5).all() and (big[:, 8 + hq * D:] == 5).all() and (lse[T:] == 5).all()
+    poisoned = qkv.clone()
+    poisoned[150:T] = float("nan")  # the second sequence
+    p = K.attention_packed(poisoned[:, :hq * D], poisoned[:, hq * D:(hq + hk) * D],
+                           poisoned[:, (hq + hk) * D:(hq + 2 * hk) * D], cu(ql), cu(ql), hq, hk)
+    assert torch.equal(p[:150], big[:150, 8:8 + hq * D]) and torch.isnan(p[150:T]).all()
+
+
+def test_attention_packed_nothing_to_do():
+    q = torch.zeros(0, 128, dtype=BF, device=DEV)
+    assert K.attention_packed(q, q, q, cu([]), cu([]), 1, 1).shape == (0, 128)
+    q = torch.ones(3, 128, dtype=BF, device=DEV)
+    o = torch.full_like(q, 2)
+    K.attention_packed(q, q, q, cu([]), cu([]), 1, 1, out=o)
+    assert (o == 2).all()
+    e = torch.zeros(0, 128, dtype=BF, device=DEV)
+    K.attention_packed(q, e, e, cu([3]), cu([0]), 1, 1, out=o)
+    assert (o == 0).all()
+
+
+def make_cache(g, lens, page, hk, D, kind, layout, spare=3):
+    need = [-(-n // page) for n in lens]
+    total = sum(need) + spare
+    order = torch.randperm(total, generator=g).to(torch.int32)
+    table = torch.full((len(lens), max(need + [1]) + 1), -7, dtype=torch.int32)  # unused entries are never read
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+    shape = (total, page, hk, D) if layout == "token" else (total, hk, page, D)
+    caches = [torch.randn(*shape, generator=g).to(DEV) for _ in range(2)]
+    scales = (None, None)
+    if kind == "fp8":
+        scales = tuple((0.005 + 0.02 * torch.rand(hk, generator=g)).to(DEV) for _ in range(2))
+        caches = [(c * 50).to(torch.float8_e4m3fn).view(torch.uint8) for c in caches]
+    else:
+        caches = [c.to(BF) for c in caches]
+    if layout != "token":
+        caches = [c.transpose(1, 2) for c in caches]
+    return table.to(DEV), caches[0], caches[1], scales
+
+
+def paged_ref(q, kc, vc, table, lens, ks, vs, scale, kind):
+    page, hk, D = kc.shape[1], kc.shape[2], kc.shape[3]
+    hq = q.shape[1] // D
+    o, tol = (torch.zeros(q.shape, dtype=torch.float64, device=DEV) for _ in range(2))
+    lse = torch.zeros(q.shape[0], hq, dtype=torch.float64, device=DEV)
+    for b, n in enumerate(lens):
+        t = torch.arange(n, device=DEV)
+        k, v = (c[table[b, t // page].long(), t % page] for c in (kc, vc))
+        if kind == "fp8":
+            k = e4m3_value(k.contiguous()) * ks.double()[:, None]
+            v = e4m3_value(v.contiguous()) * vs.double()[:, None]
+        for h in range(hq):
+            g = h // (hq // hk)
+            c = slice(h * D, (h + 1) * D)
+            o[b:b + 1, c], tol[b:b + 1, c], lse[b:b + 1, h] = attend_ref(
+                q[b:b + 1, c], k[:, g], v[:, g], None, scale, 2.0 ** -11 if kind == "fp8" else 2.0 ** -8)
+    return o, tol, lse
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,hq,hk,page,layout", [
+    ([1], 1, 1, 16, "token"),
+    ([1000], 32, 8, 16, "token"),
+    ([0, 1, 16, 17, 63, 64, 65, 0], 8, 2, 16, "token"),
+    ([5000, 3, 777], 24, 1, 64, "head"),      # more than 16 query heads per key head
+    ([300, 200], 12, 1, 24, "token"),         # 9 to 16 heads; pages that end inside a block
+    ([129, 40], 6, 3, 1, "head"),
+    ([2049] * 5 + [0] + [31] * 3, 16, 4, 128, "head"),
+    ([20000, 1], 4, 2, 32, "token"),          # split over many SMs
+    ([37] * 300, 4, 4, 16, "token"),          # many short sequences
+    ([0, 0], 2, 1, 16, "token"),
+])
+def test_attention_paged(kind, D, lens, hq, hk, page, layout):
+    g = gen(sum(lens) + D + hq)
+    table, kc, vc, (ks, vs) = make_cache(g, lens, page, hk, D, kind, layout)
+    q = randn(g, len(lens), hq * D)
+    lse = torch.zeros(len(lens), hq, device=DEV)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    o = K.attention_paged(q, kc, vc, table, n, k_scale=ks, v_scale=vs, lse=lse)
+    want, tol, wl = paged_ref(q, kc, vc, table, lens, ks, vs, D ** -0.5, kind)
+    assert ((o.double() - want).abs() <= tol).all(), ((o.double() - want).abs() / tol).max().item()
+    close_lse(lse, wl)
+    assert torch.equal(o, K.attention_paged(q, kc, vc, table, n, k_scale=ks, v_scale=vs))  # deterministic
+
+
+def test_attention_paged_large_queries_fp8():
+    """q far outside fp16's range: the row's power of two keeps it inside."""
+    g = gen(5)
+    table, kc, vc, (ks, vs) = make_cache(g, [100], 16, 1, 128, "fp8", "token")
+    q = randn(g, 1, 2 * 128, mul=1e8)
+    o = K.attention_paged(q, kc, vc, table, torch.tensor([100], dtype=torch.int32, device=DEV), k_scale=ks, v_scale=vs,
+                          scale=1e-9)
+    want, tol, _ = paged_ref(q, kc, vc, table, [100], ks, vs, 1e-9, "fp8")
+    assert ((o.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_attention_paged_garbage_behind_the_length(kind):
+    """Slots behind a sequence's last token hold NaN (bf16 and E4M3 have one): the result does not see them."""
+    g = gen(6)
+    lens = [5, 70]
+    table, kc, vc, (ks, vs) = make_cache(g, lens, 16, 2, 64, kind, "token")
+    q = randn(g, 2, 4 * 64)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    o = K.attention_paged(q, kc, vc, table, n, k_scale=ks, v_scale=vs)
+    nan = float("nan") if kind == "bf16" else 0x7F
+    for b, m in enumerate(lens):
+        last = table[b, (m - 1) // 16].long()
+        kc[last, (m - 1) % 16 + 1:] = nan
+        vc[last, (m - 1) % 16 + 1:] = nan
+    assert torch.equal(o, K.attention_paged(q, kc, vc, table, n, k_scale=ks, v_scale=vs))
+
+
+def test_attention_paged_bad_pages_and_lengths_are_left_out():
+    g = gen(7)
+    lens = [64, 48]
+    table, kc, vc, _ = make_cache(g, lens, 16, 1, 128, "bf16", "token")
+    q = randn(g, 2, 2 * 128)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    bad = table.clone()
+    bad[0, 1], bad[0, 3] = -1, 10 ** 6
+    o = K.attention_paged(q, kc, vc, bad, n)
+    with pytest.raises(_lib.QiB200DeviceError, match="out of range"):
+        _lib.raise_on_device_error()
+    keep = table.clone()
+    keep[0, 1] = table[0, 2]
+    want = K.attention_paged(q, kc, vc, keep, torch.tensor([32, 48], dtype=torch.int32, device=DEV))
+    # the same 32 keys in another grouping: both within half a step of bf16 (and of its P) of the exact result
+    assert ((o.float() - want.float()).abs() <= 2.0 ** -5).all()
+    assert torch.equal(o[1], want[1])
+    long = torch.tensor([64, 10 ** 9], dtype=torch.int32, device=DEV)  # behind the table: cut to its 5 columns
+    full = torch.cat([table, table[:, :0]], 1)
+    full[:, 3:] = full[:, :1]
+    o2 = K.attention_paged(q, kc, vc, full, long)
+    with pytest.raises(_lib.QiB200DeviceError, match="out of range"):
+        _lib.raise_on_device_error()
+    cut = torch.tensor([64, 16 * full.shape[1]], dtype=torch.int32, device=DEV)
+    assert torch.equal(o2, K.attention_paged(q, kc, vc, full, cut))
+    _lib.raise_on_device_error()
+
+
+# ---------------------------------------------------------------------------
+# streams, graphs, refusals, and all of them together
+# ---------------------------------------------------------------------------
+
+
+def test_side_stream_and_graph_replay():
+    """All operators captured twice into graphs with their own workspaces, replayed on two streams at once with new
+    inputs, give the eager results."""
+    g = gen(8)
+    lens, hq, hk, D = [700, 3000], 8, 2, 128
+    table, kc, vc, _ = make_cache(g, lens, 16, hk, D, "bf16", "token")
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    freqs, axes = K.rope_axes_frequencies((D // 2,), shared=True, device=DEV)
+    w = randn(g, hq * D)
+    pos = torch.arange(2, device=DEV)
+    c = cu([1, 1])
+
+    def chain(x):
+        q8, s8 = K.rms_norm_quant(_lib.KIND_FP8_E4M3, x, w)
+        q, _ = K.rope_axes(x, None, pos, freqs, axes, D)
+        a = K.attention_paged(q, kc, vc, table, n)
+        return a, q8, s8, K.attention_packed(a, a[:, :hk * D], a[:, hk * D:2 * hk * D], c, c, hq, hk)
+
+    xs = [randn(g, 2, hq * D) for _ in range(4)]
+    want = [chain(x) for x in xs]
+    graphs, ins, outs = [], [], []
+    for i in range(2):
+        x = xs[i].clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o = chain(x)
+        graphs.append(graph), ins.append(x), outs.append(o)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for base in (0, 2):
+        for i in range(2):
+            ins[i].copy_(xs[base + i])
+        torch.cuda.synchronize()
+        for rep in range(3):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            for a, b in zip(outs[i], want[base + i]):
+                assert torch.equal(a, b)
+    with torch.cuda.stream(streams[0]):
+        got = chain(xs[3])
+    streams[0].synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[3]))
+
+
+def test_refusals():
+    x = torch.zeros(4, 256, dtype=BF, device=DEV)
+    w = torch.ones(256, dtype=BF, device=DEV)
+    bad = [
+        lambda: K.rms_norm_quant(_lib.KIND_INT8, x.float(), w),
+        lambda: K.rms_norm_quant(_lib.KIND_INT8, x[:, :250], w[:250]),
+        lambda: K.rms_norm_quant(_lib.KIND_INT8, x[:, 1:249], w[:248]),
+        lambda: K.rms_norm_quant(_lib.KIND_INT8, x, w[:128]),
+        lambda: K.rms_norm_quant(_lib.KIND_INT8, x, w, x[:3]),
+        lambda: K.rms_norm_quant(_lib.KIND_INT8, x, w, x_out=x),
+        lambda: K.rms_norm_quant(_lib.KIND_BF16, x, w),
+        lambda: K.rms_norm_quant(7, x, w),
+        lambda: K.rms_norm_quant(_lib.KIND_INT8, x.cpu(), w),
+        lambda: K.rms_norm_quant(_lib.KIND_INT8, x, w, q=torch.zeros(4, 256, dtype=torch.uint8, device=DEV)),
+        lambda: K.rms_norm_quant(_lib.KIND_INT8, torch.zeros(1, 16392, dtype=BF, device=DEV),
+                                 torch.zeros(16392, dtype=BF, device=DEV)),
+    ]
+    f, a = K.rope_axes_frequencies((64,), device=DEV)
+    pos = torch.zeros(4, dtype=torch.int32, device=DEV)
+    kc = torch.zeros(2, 4, 1, 128, dtype=BF, device=DEV)
+    k1 = x[:, :128]
+    slots = torch.arange(4, device=DEV)
+    bad += [
+        lambda: K.rope_axes_frequencies((8, 0), device=DEV),
+        lambda: K.rope_axes(x, None, pos[:3], f, a, 128),
+        lambda: K.rope_axes(x, None, pos.float(), f, a, 128),
+        lambda: K.rope_axes(x, None, pos, f.float(), a, 128),
+        lambda: K.rope_axes(x, None, pos, f[:60], a[:60], 128),
+        lambda: K.rope_axes(x, None, pos, f, a, 64),       # 64 pairs do not fit a head of 64
+        lambda: K.rope_axes(x, None, pos, f, a, 96),       # 256 columns are no whole number of heads
+        lambda: K.rope_axes_store(x, k1, k1, pos, f, a, 128, kc, kc[:1], slots),
+        lambda: K.rope_axes_store(x, k1, None, pos, f, a, 128, kc, kc, slots),
+        lambda: K.rope_axes_store(x, k1, k1, pos, f, a, 128, kc, kc, slots[:3]),
+        lambda: K.rope_axes_store(x, x, x, pos, f, a, 128, kc, kc, slots),
+        lambda: K.rope_axes_store(x, k1, k1, pos, f, a, 128, kc.to(torch.uint8), kc.to(torch.uint8), slots),
+        lambda: K.rope_axes_store(x, k1, k1, pos, f, a, 128, kc, kc, slots, k_scale=torch.ones(1, device=DEV)),
+        lambda: K.rope_axes_store(x, k1, k1, pos, f, a, 128, kc.half(), kc.half(), slots),
+    ]
+    c = cu([4])
+    bad += [
+        lambda: K.attention_packed(x, x, x, c, c, 4, 3),
+        lambda: K.attention_packed(x, x, x, c, c, 2, 1),
+        lambda: K.attention_packed(x, x, x, c, c, 1, 1),   # head dim 256
+        lambda: K.attention_packed(x, x, x[:3], c, c, 2, 2),
+        lambda: K.attention_packed(x, x, x, c.long(), c.long(), 2, 2),
+        lambda: K.attention_packed(x, x, x, c, cu([2, 2]), 2, 2),
+        lambda: K.attention_packed(x, x, x, c, c, 2, 2, scale=0.0),
+        lambda: K.attention_packed(x, x, x, c, c, 2, 2, scale=float("nan")),
+        lambda: K.attention_packed(x, x, x, c, c, 2, 2, lse=torch.zeros(4, 3, device=DEV)),
+        lambda: K.attention_packed(x, x, x, c, c, 2, 2, out=torch.zeros(3, 256, dtype=BF, device=DEV)),
+    ]
+    t, n = torch.zeros(4, 2, dtype=torch.int32, device=DEV), torch.ones(4, dtype=torch.int32, device=DEV)
+    bad += [
+        lambda: K.attention_paged(x, kc, kc, t[:3], n),
+        lambda: K.attention_paged(x, kc, kc, t.long(), n),
+        lambda: K.attention_paged(x, kc, kc, t, n[:3]),
+        lambda: K.attention_paged(x, kc, kc, t, n.long()),
+        lambda: K.attention_paged(x, kc[..., :96], kc[..., :96], t, n),
+        lambda: K.attention_paged(x, kc[..., 4:68], kc[..., 4:68], t, n),
+        lambda: K.attention_paged(x, kc, kc, t, n, v_scale=torch.ones(1, device=DEV)),
+        lambda: K.attention_paged(x, kc.view(torch.uint8), kc.view(torch.uint8), t, n),
+        lambda: K.attention_paged(x, kc[:0], kc[:0], t, n),
+        lambda: K.attention_paged(x, kc, kc, t, n, scale=-1.0),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises((ValueError, _lib.QiB200Error)):
+            call()
+            print("not refused:", i)
+
+
+def test_decoder_block_prompt_then_tokens():
+    """The operators as they are used: prompts through norm -> INT8 q/k/v linear -> rotary + cache -> packed attention
+    -> INT8 output linear with residual, then three single tokens through the paged path.  Every step is checked against
+    its 64-bit form on the framework's own inputs of that step, and the paged result against packed attention over the
+    whole sequence."""
+    g = gen(9)
+    hid, hq, hk, D, page = 512, 8, 2, 64, 16
+    lens = [75, 130, 1]
+    width = (hq + 2 * hk) * D
+
+    def int8_weight(n, k):
+        w = torch.randint(-127, 128, (n, k), generator=g).to(torch.int8).to(DEV)
+        return w, torch.full((n,), 0.7 / 127 / k ** 0.5, device=DEV)
+
+    wqkv, sqkv = int8_weight(width, hid)
+    wo, so = int8_weight(hid, hq * D)
+    norm = randn(g, hid, mul=0.1) + 1
+    freqs, axes = K.rope_axes_frequencies((8, 12, 12), shared=True, device=DEV)
+    pages = sum(-(-(n + 3) // page) for n in lens)
+    kc, vc = (torch.zeros(pages, page, hk, D, dtype=BF, device=DEV) for _ in range(2))
+    table = torch.zeros(len(lens), 10, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(lens):
+        m = -(-(n + 3) // page)
+        table[b, :m] = torch.arange(at, at + m)
+        at += m
+
+    def layer(x, y, pos, slots):
+        q8, s8 = K.rms_norm_quant(_lib.KIND_INT8, x, norm, y)
+        check_norm(_lib.KIND_INT8, None, norm, None, 1e-6, q8, s8, x)
+        qkv = K.gemm(_lib.KIND_INT8, q8, wqkv, s8, sqkv)
+        q, k, v = qkv[:, :hq * D], qkv[:, hq * D:(hq + hk) * D], qkv[:, (hq + hk) * D:]
+        K.rope_axes_store(q, k, v, pos, freqs, axes, D, kc, vc, slots, interleaved=False, out_q=q, out_k=k)
+        return q, k, v
+
+    x = randn(g, sum(lens), hid)
+    y = randn(g, sum(lens), hid)
+    pos = torch.cat([torch.arange(n) for n in lens]).expand(3, -1).contiguous().to(DEV)
+    seq = torch.cat([torch.full((n,), b) for b, n in enumerate(lens)])
+    slot = lambda b, t: table[b, t // page].long() * page + t % page
+    q, k, v = layer(x, y, pos, slot(seq, pos[0].cpu()).to(DEV))
+    c = cu(lens)
+    o = K.attention_packed(q, k, v, c, c, hq, hk)
+    want, tol, _ = packed_ref(q, k, v, lens, lens, hq, hk, D, True, D ** -0.5)
+    assert ((o.double() - want).abs() <= tol).all()
+    y = K.int8_linear(o, wo, so)
+    history = [(list(torch.split(k, lens)), list(torch.split(v, lens)))]
+    ks, vs = history[0]
+    last = c[1:].long() - 1
+    xt, yt = x[last].contiguous(), y[last].contiguous()
+    for step in range(3):
+        now = torch.tensor([n + step for n in lens])
+        q, k, v = layer(xt, yt, now.expand(3, -1).contiguous().to(DEV), slot(torch.arange(3), now).to(DEV))
+        n = (now + 1).to(torch.int32).to(DEV)
+        o = K.attention_paged(q, kc, vc, table.to(DEV), n)
+        ks = [torch.cat([a, k[b:b + 1]]) for b, a in enumerate(ks)]
+        vs = [torch.cat([a, v[b:b + 1]]) for b, a in enumerate(vs)]
+        total = [a.shape[0] for a in ks]
+        want, tol, _ = packed_ref(q, torch.cat(ks), torch.cat(vs), [1] * 3, total, hq, hk, D, True, D ** -0.5)
+        assert ((o.double() - want).abs() <= tol).all()
+        same = K.attention_packed(q, torch.cat(ks), torch.cat(vs), cu([1] * 3), cu(total), hq, hk)
+        assert ((same.double() - want).abs() <= tol).all()
+        yt = K.int8_linear(o, wo, so)
