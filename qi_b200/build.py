@@ -78,7 +78,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
     import torch
     from torch.utils import cpp_extension as ce
 
-    deps = [TORCH_OPS_SRC, ROOT / "include" / "qi_b200.h", LIB]
+    deps = [*CSRC.glob("torch_ops*"), ROOT / "include" / "qi_b200.h", LIB]
     if not force and TORCH_OPS_LIB.exists() and all(p.stat().st_mtime <= TORCH_OPS_LIB.stat().st_mtime for p in deps):
         return TORCH_OPS_LIB
     build(force=False)

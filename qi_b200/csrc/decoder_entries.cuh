@@ -177,6 +177,8 @@ int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk
     if (cache != nullptr && (ldv < wk || ldv % 8)) return QI_B200_ESHAPE;
     if (cache != nullptr && !aligned16(v)) return QI_B200_EALIGN;
   }
+  if (cache != nullptr)
+    if (int rc = check_paged_cache(cache, kv_heads, head_dim)) return rc;
   DeviceInfo* di = nullptr;
   if (int rc = device_info(&di)) return rc;
   RopeAxesParams p = {};
@@ -202,7 +204,6 @@ int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk
   p.M = M;
   int kind = 0;
   if (cache != nullptr) {
-    if (int rc = check_paged_cache(cache, kv_heads, head_dim)) return rc;
     kind = cache->fp8 ? 2 : 1;
     p.cache[0] = cache->k;
     p.cache[1] = cache->v;

@@ -15,6 +15,7 @@
 #include <optional>
 
 #include "../../include/qi_b200.h"
+#include "torch_ops_decoder.h"
 
 namespace {
 

@@ -10,9 +10,11 @@ so every function here is safe inside ``torch.cuda.graph`` capture.
 
 from __future__ import annotations
 
+import re
+
 import torch
 
-from . import _lib
+from . import _lib, torch_ops
 
 _U8 = torch.uint8
 
@@ -539,29 +541,25 @@ def fp8_linear(x_bf16_2d: torch.Tensor, weight_fp8: torch.Tensor, weight_scale: 
 # ---------------------------------------------------------------------------
 
 
-def _launch(dev: torch.device, fn_name: str, *args) -> None:
-    """The C call with ``dev`` as the current device (its tensors' own) on dev's current stream."""
-    if torch.cuda.current_device() == dev.index:
-        _lib.call(fn_name, *args, _stream(dev))
-        return
-    with torch.cuda.device(dev):
-        _lib.call(fn_name, *args, _stream(dev))
+_OPS: dict = {}
+_STATUS = re.compile(r"^(\w+) failed with status (\d+)")
 
 
-def _rows(t: torch.Tensor, name: str, width: int, rows: int | None = None, device=None) -> int:
-    """Check a bf16 [rows, width] block (column slices of wider rows allowed) and return its row stride."""
-    if not t.is_cuda or t.dtype != torch.bfloat16 or t.dim() != 2:
-        raise ValueError(f"{name} must be a 2-D bf16 CUDA tensor.")
-    if t.shape[1] != width or (rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {width}], got {tuple(t.shape)}.")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}.")
-    if t.numel() == 0:
-        return width
-    ld = t.stride(0) if t.shape[0] > 1 else -(-width // 8) * 8
-    if t.stride(1) != 1 or ld < width or ld % 8 or t.data_ptr() % 16:
-        raise ValueError(f"{name} must have unit column stride, rows that do not overlap and 16-byte aligned rows.")
-    return ld
+def _op(name: str, *args):
+    """Call the compiled torch operator ``qi_b200::<name>``, which checks the
+    arguments (``ValueError``), allocates and launches; a status of the library
+    comes back as the exceptions of ``_lib.check``."""
+    op = _OPS.get(name)
+    if op is None:
+        torch_ops.load()
+        op = _OPS[name] = getattr(torch.ops.qi_b200, name).default
+    try:
+        return op(*args)
+    except RuntimeError as e:
+        m = _STATUS.match(str(e))
+        if m is None:
+            raise
+        _lib.check(m.group(1), int(m.group(2)))
 
 
 def rms_norm_quant(kind: int, x: torch.Tensor, weight: torch.Tensor, y: torch.Tensor | None = None, *,
@@ -577,44 +575,7 @@ def rms_norm_quant(kind: int, x: torch.Tensor, weight: torch.Tensor, y: torch.Te
     E4M3 codes [M, D], fp32 [M]), the operands of ``gemm``; ``KIND_BF16``
     returns (None, None) and needs ``xn``.  ``xn`` [M, D] receives the
     normalized row in bf16.  D % 8 == 0, D <= 16384."""
-    if kind not in (_lib.KIND_INT8, _lib.KIND_FP8_E4M3, _lib.KIND_BF16):
-        raise ValueError(f"unknown kind {kind}.")
-    if x.dim() != 2:
-        raise ValueError(f"x must be 2-D, got shape {tuple(x.shape)}.")
-    M, D = x.shape
-    dev = x.device
-    ldx = _rows(x, "x", D)
-    if D == 0 or D % 8 or D > 16384:
-        raise ValueError(f"rms_norm_quant needs D % 8 == 0 and 0 < D <= 16384, got {D}.")
-    _check(weight, "weight", torch.bfloat16, device=dev)
-    if weight.numel() != D:
-        raise ValueError(f"weight must have {D} values.")
-    if y is None:
-        if x_out is not None:
-            raise ValueError("x_out needs y: without a residual the rows of x do not change.")
-        ldy, ld_out = 0, 0
-    else:
-        ldy = _rows(y, "y", D, M, dev)
-        x_out = x if x_out is None else x_out
-        ld_out = _rows(x_out, "x_out", D, M, dev)
-    if xn is not None:
-        _check(xn, "xn", torch.bfloat16, 2, dev)
-        if tuple(xn.shape) != (M, D):
-            raise ValueError(f"xn must be [{M}, {D}].")
-    if kind == _lib.KIND_BF16:
-        if xn is None or q is not None or s is not None:
-            raise ValueError("KIND_BF16 writes xn only.")
-    else:
-        dt = torch.int8 if kind == _lib.KIND_INT8 else torch.uint8
-        q = q if q is not None else torch.empty((M, D), dtype=dt, device=dev)
-        s = s if s is not None else torch.empty((M,), dtype=torch.float32, device=dev)
-        _check(q, "q", dt, 2, dev)
-        _check(s, "s", torch.float32, 1, dev)
-        if tuple(q.shape) != (M, D) or s.numel() != M:
-            raise ValueError(f"q must be [{M}, {D}] and s [{M}].")
-    _launch(dev, "qi_b200_rms_norm_quant", kind, _ptr(x), ldx, _ptr(y), ldy, _ptr(x_out), ld_out, _ptr(weight),
-            _ptr(q), _ptr(s), _ptr(xn), M, D, float(eps))
-    return q, s
+    return _op("rms_norm_quant", kind, x, weight, y, eps, x_out, q, s, xn)
 
 
 def rope_axes_frequencies(sections, theta: float = 10000.0, shared: bool = False, device="cuda"):
@@ -635,85 +596,6 @@ def rope_axes_frequencies(sections, theta: float = 10000.0, shared: bool = False
             torch.tensor(axes, dtype=torch.int32, device=device))
 
 
-def _index(t: torch.Tensor, name: str, device) -> int:
-    """Check an int32 / int64 index tensor; 1 for int64."""
-    _check(t, name, (torch.int32, torch.int64), device=device)
-    return int(t.dtype == torch.int64)
-
-
-def _cache(k_cache, v_cache, k_scale, v_scale, kv_heads: int, head_dim: int, dev) -> "_lib.PagedCache":
-    """Check a [pages, page_size, kv_heads, head_dim] cache pair (any strides but the last) and describe it."""
-    dt = k_cache.dtype
-    fp8 = dt in (torch.uint8, torch.float8_e4m3fn)
-    if not fp8 and dt != torch.bfloat16:
-        raise ValueError(f"the cache must be bf16, uint8 (E4M3 codes) or float8_e4m3fn, got {dt}.")
-    c = _lib.PagedCache()
-    for i, (t, name) in enumerate(((k_cache, "k_cache"), (v_cache, "v_cache"))):
-        if t.dim() != 4 or t.dtype != dt or t.device != dev or t.shape != k_cache.shape:
-            raise ValueError(f"{name} must be [pages, page_size, kv_heads, head_dim], both caches alike, on {dev}.")
-        if t.shape[2] != kv_heads or t.shape[3] != head_dim:
-            raise ValueError(f"{name} must hold {kv_heads} heads of {head_dim}, got {tuple(t.shape)}.")
-        st = [t.stride(d) if t.shape[d] > 1 else 0 for d in range(3)]
-        if t.stride(3) != 1 or any(v * t.element_size() % 16 for v in st) or t.data_ptr() % 16:
-            raise ValueError(f"{name} must have unit stride inside a head and 16-byte aligned heads.")
-        c.page_stride[i], c.slot_stride[i], c.head_stride[i] = st
-    c.k, c.v = k_cache.data_ptr(), v_cache.data_ptr()
-    c.pages, c.page_size, c.fp8 = k_cache.shape[0], k_cache.shape[1], int(fp8)
-    if c.page_size == 0:
-        raise ValueError("the cache's pages must hold at least one token.")
-    for i, (s, name) in enumerate(((k_scale, "k_scale"), (v_scale, "v_scale"))):
-        if not fp8:
-            if s is not None:
-                raise ValueError(f"{name} belongs to an E4M3 cache.")
-            continue
-        if s is None:
-            raise ValueError(f"an E4M3 cache needs {name}.")
-        _check(s, name, torch.float32, device=dev)
-        if s.numel() not in (1, kv_heads):
-            raise ValueError(f"{name} must have 1 or {kv_heads} values.")
-        c.scale[i] = s.data_ptr()
-        c.scale_per_head[i] = int(s.numel() > 1)
-    return c
-
-
-def _rope(q, k, v, positions, freqs, axes, head_dim, interleaved, out_q, out_k, cache, slots, slots64):
-    import ctypes
-
-    dev = q.device
-    if head_dim <= 0 or head_dim % 16 or head_dim > 512 or q.dim() != 2 or q.shape[1] % head_dim or q.shape[1] == 0:
-        raise ValueError(f"q must be [M, heads * head_dim] with head_dim % 16 == 0 and <= 512 (head_dim {head_dim}).")
-    M, heads = q.shape[0], q.shape[1] // head_dim
-    ldq = _rows(q, "q", q.shape[1])
-    pos = positions if positions.dim() == 2 else positions.unsqueeze(0)
-    pos64 = _index(pos, "positions", dev)
-    if pos.dim() != 2 or pos.shape[1] != M or pos.shape[0] == 0:
-        raise ValueError(f"positions must be [axes, {M}], got {tuple(positions.shape)}.")
-    _check(freqs, "freqs", torch.float64, 1, dev)
-    _check(axes, "axes", torch.int32, 1, dev)
-    P = freqs.numel()
-    if axes.numel() != P or P == 0 or P % 8 or 2 * P > head_dim:
-        raise ValueError(f"freqs and axes must have the same number of pairs, a multiple of 8 up to {head_dim // 2}.")
-    if out_q is None:
-        out_q = torch.empty((M, q.shape[1]), dtype=torch.bfloat16, device=dev)
-    ldq_out = _rows(out_q, "out_q", q.shape[1], M, dev)
-    ldk = ldv = ldk_out = kv_heads = 0
-    if k is not None:
-        if k.dim() != 2 or k.shape[1] % head_dim or k.shape[1] == 0:
-            raise ValueError("k must be [M, kv_heads * head_dim].")
-        kv_heads = k.shape[1] // head_dim
-        ldk = _rows(k, "k", k.shape[1], M, dev)
-        if cache is None and out_k is None:
-            out_k = torch.empty((M, k.shape[1]), dtype=torch.bfloat16, device=dev)
-        if out_k is not None:
-            ldk_out = _rows(out_k, "out_k", k.shape[1], M, dev)
-        if cache is not None:
-            ldv = _rows(v, "v", k.shape[1], M, dev)
-    _launch(dev, "qi_b200_rope_axes", _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, _ptr(out_q), ldq_out, _ptr(out_k),
-            ldk_out, _ptr(pos), pos64, _ptr(freqs), _ptr(axes), P, pos.shape[0], int(bool(interleaved)), M, heads,
-            kv_heads, head_dim, None if cache is None else ctypes.byref(cache), _ptr(slots), slots64)
-    return out_q, out_k
-
-
 def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs: torch.Tensor,
               axes: torch.Tensor, head_dim: int, *, interleaved: bool = True, out_q: torch.Tensor | None = None,
               out_k: torch.Tensor | None = None):
@@ -726,7 +608,7 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, 
     (2i, 2i+1) (``interleaved``, as the DiT's) or (i, i + pairs); elements
     behind the last pair pass unchanged.  Returns (q, k) rotated; ``out_q`` /
     ``out_k`` may be ``q`` / ``k`` themselves."""
-    return _rope(q, k, None, positions, freqs, axes, head_dim, interleaved, out_q, out_k, None, None, 0)
+    return _op("rope_axes", q, k, positions, freqs, axes, head_dim, interleaved, out_q, out_k)
 
 
 def rope_axes_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor,
@@ -744,30 +626,8 @@ def rope_axes_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     [M]: page * page_size + place of each row, all different; a negative slot
     writes nothing (padding rows), one outside the cache writes nothing and is
     reported by ``_lib.raise_on_device_error``.  Returns the rotated q."""
-    if k is None or v is None:
-        raise ValueError("rope_axes_store needs k and v.")
-    if head_dim <= 0 or k.dim() != 2 or k.shape[1] % head_dim:
-        raise ValueError("k must be [M, kv_heads * head_dim].")
-    cache = _cache(k_cache, v_cache, k_scale, v_scale, k.shape[1] // head_dim, head_dim, q.device)
-    slots64 = _index(slots, "slots", q.device)
-    if slots.dim() != 1 or slots.numel() != q.shape[0]:
-        raise ValueError(f"slots must be [{q.shape[0]}], got {tuple(slots.shape)}.")
-    return _rope(q, k, v, positions, freqs, axes, head_dim, interleaved, out_q, out_k, cache, slots, slots64)[0]
-
-
-def _attention_args(head_dim: int, heads: int, kv_heads: int, scale: float | None, lse, rows: int, dev) -> float:
-    if head_dim not in (64, 128):
-        raise ValueError(f"head_dim must be 64 or 128, got {head_dim}.")
-    if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
-        raise ValueError(f"{heads} query heads do not share {kv_heads} key heads evenly.")
-    if lse is not None:
-        _check(lse, "lse", torch.float32, 2, dev)
-        if tuple(lse.shape) != (rows, heads):
-            raise ValueError(f"lse must be [{rows}, {heads}].")
-    scale = float(head_dim ** -0.5 if scale is None else scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive and finite, got {scale}.")
-    return scale
+    return _op("rope_axes_store", q, k, v, positions, freqs, axes, head_dim, k_cache, v_cache, slots, interleaved,
+               k_scale, v_scale, out_q, out_k)
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
@@ -783,41 +643,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     bf16 (or writes ``out``; its rows outside every sequence stay as they
     were).  ``lse`` fp32 [Tq, heads] receives the log of the softmax sums.
     Default scale 1 / sqrt(D)."""
-    dev = q.device
-    if q.dim() != 2 or heads <= 0 or q.shape[1] % heads:
-        raise ValueError(f"q must be [Tq, {heads} * head_dim].")
-    D = q.shape[1] // heads
-    scale = _attention_args(D, heads, kv_heads, scale, lse, q.shape[0], dev)
-    ldq = _rows(q, "q", heads * D)
-    ldk = _rows(k, "k", kv_heads * D, None, dev)
-    ldv = _rows(v, "v", kv_heads * D, k.shape[0], dev)
-    _check(cu_q, "cu_q", torch.int32, 1, dev)
-    _check(cu_k, "cu_k", torch.int32, 1, dev)
-    if cu_q.numel() == 0 or cu_q.numel() != cu_k.numel():
-        raise ValueError("cu_q and cu_k must be int32 [sequences + 1].")
-    if out is None:
-        out = torch.empty((q.shape[0], heads * D), dtype=torch.bfloat16, device=dev)
-    ldo = _rows(out, "out", heads * D, q.shape[0], dev)
-    _launch(dev, "qi_b200_attention_packed", _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, _ptr(out), ldo, _ptr(lse),
-            _ptr(cu_q), _ptr(cu_k), cu_q.numel() - 1, q.shape[0], k.shape[0], heads, kv_heads, D, int(bool(causal)),
-            scale)
-    return out
-
-
-_PAGED_WS: dict = {}
-
-
-def _paged_workspace(dev: torch.device, head_dim: int) -> torch.Tensor:
-    """Workspace of one ``attention_paged`` call from torch's caching allocator (its size is a property of the device)."""
-    key = (dev.index, head_dim)
-    n = _PAGED_WS.get(key)
-    if n is None:
-        import ctypes
-        nb = ctypes.c_size_t(0)
-        with torch.cuda.device(dev):
-            _lib.call("qi_b200_attention_paged_workspace_bytes", head_dim, ctypes.byref(nb))
-        n = _PAGED_WS[key] = int(nb.value)
-    return torch.empty((n,), dtype=_U8, device=dev)
+    return _op("attention_packed", q, k, v, cu_q, cu_k, heads, kv_heads, causal, scale, out, lse)
 
 
 def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor,
@@ -835,31 +661,4 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     behind the table, is left out and reported by
     ``_lib.raise_on_device_error``.  Returns [B, heads * D] bf16 (or writes
     ``out``); ``lse`` fp32 [B, heads] receives the log of the softmax sums."""
-    import ctypes
-
-    dev = q.device
-    if k_cache.dim() != 4:
-        raise ValueError("k_cache must be [pages, page_size, kv_heads, head_dim].")
-    kv_heads, D = k_cache.shape[2], k_cache.shape[3]
-    if q.dim() != 2 or D == 0 or q.shape[1] % D:
-        raise ValueError(f"q must be [B, heads * {D}].")
-    B, heads = q.shape[0], q.shape[1] // D
-    scale = _attention_args(D, heads, kv_heads, scale, lse, B, dev)
-    ldq = _rows(q, "q", heads * D)
-    cache = _cache(k_cache, v_cache, k_scale, v_scale, kv_heads, D, dev)
-    if not pages.is_cuda or pages.dtype != torch.int32 or pages.dim() != 2 or pages.device != dev \
-            or pages.shape[0] != B or (pages.shape[1] > 1 and pages.stride(1) != 1):
-        raise ValueError(f"pages must be int32 [{B}, max_pages] on {dev} with unit column stride.")
-    _check(lengths, "lengths", torch.int32, 1, dev)
-    if lengths.numel() != B:
-        raise ValueError(f"lengths must be [{B}].")
-    if B > 65535:
-        raise ValueError("attention_paged takes at most 65535 sequences.")
-    if out is None:
-        out = torch.empty((B, heads * D), dtype=torch.bfloat16, device=dev)
-    ldo = _rows(out, "out", heads * D, B, dev)
-    ws = _paged_workspace(dev, D)
-    _launch(dev, "qi_b200_attention_paged", _ptr(q), ldq, ctypes.byref(cache), _ptr(pages),
-            pages.stride(0) if B > 1 else pages.shape[1], pages.shape[1], _ptr(lengths), _ptr(out), ldo, _ptr(lse), B,
-            heads, kv_heads, D, scale, _ptr(ws), ws.numel())
-    return out
+    return _op("attention_paged", q, k_cache, v_cache, pages, lengths, scale, k_scale, v_scale, out, lse)

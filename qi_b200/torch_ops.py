@@ -1,6 +1,9 @@
 """Torch operators over the C ABI: ``torch.ops.qi_int8_w8a8.linear`` with the
 reference's schema (``src/qi/quantization/csrc/int8_w8a8/bindings.cpp:159-165``)
-and ``torch.ops.qi_b200.{int8_linear, fp8_linear, w4a16_linear}``.
+and ``torch.ops.qi_b200.{int8_linear, fp8_linear, w4a16_linear}``, and the
+decoder-block operators ``torch.ops.qi_b200.{rms_norm_quant, rope_axes,
+rope_axes_store, attention_packed, attention_paged}`` (documented in
+``qi_b200.kernels``, which calls them).
 
 They live in the in-tree ``libqi_b200_torch.so`` (``qi_b200/csrc/torch_ops.cpp``,
 built by ``python -m qi_b200.build``), which links the in-tree
