@@ -21,9 +21,9 @@
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of tile 0 and 1, warp 8 TMA,
 // warp 9 MMA (10 and 11 fill up their warpgroup).  A softmax thread holds a
-// whole row of S, so the softmax warpgroups take 208 registers a thread and
-// the third leaves them all but 80 (of 168 at launch: 256 x 208 + 128 x 80 =
-// 63,488 of 64,512).  CTAs are persistent; each takes every gridDim.x-th item, longest
+// whole row of S, so the softmax warpgroups take 216 registers a thread and
+// the third leaves them all but 72 (of 168 at launch: 256 x 216 + 128 x 72 =
+// 64,512, all of them).  CTAs are persistent; each takes every gridDim.x-th item, longest
 // items first, the direction alternating from round to round.  The order is a
 // function of cu_q alone: level L (the L-th query block of every sequence that
 // has one) from the last to the first, so no list of items is stored.
@@ -110,10 +110,10 @@ struct PackedItem {
 // The items of one CTA in order; every warp walks the same sequence.
 struct PackedSched {
   const PackedParams& p;
-  int lane, per_seq_level, rows_per_item, heads_items;
+  int lane, rows_per_item, heads_items;
   int level, chunk;
-  long long base;      // items before the current (level, chunk)
-  long long round;
+  int base;            // items before the current (level, chunk)
+  int round;
   unsigned mask;       // active sequences of the chunk
   int blocks0;         // query blocks of sequence `lane` (chunk 0)
 
@@ -144,11 +144,11 @@ struct PackedSched {
     mask = __ballot_sync(0xffffffffu, blocks0 > level);
   }
   __device__ __forceinline__ bool next(PackedItem& it) {
-    const long long G = gridDim.x;
-    const long long target = round * G + ((round & 1) ? G - 1 - blockIdx.x : blockIdx.x);
+    const int G = gridDim.x;
+    const int target = round * G + ((round & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
     if (level < 0) return false;
-    while (target >= base + static_cast<long long>(__popc(mask)) * heads_items) {
-      base += static_cast<long long>(__popc(mask)) * heads_items;
+    while (target >= base + __popc(mask) * heads_items) {
+      base += __popc(mask) * heads_items;
       chunk += 32;
       if (chunk >= p.n_seq) {
         chunk = 0;
@@ -157,7 +157,7 @@ struct PackedSched {
       mask = __ballot_sync(0xffffffffu, (chunk == 0 ? blocks0 : seq_blocks(chunk + lane)) > level);
     }
     ++round;
-    const int idx = static_cast<int>(target - base);
+    const int idx = target - base;
     const int nth = idx / heads_items, hi = idx - nth * heads_items;
     unsigned mm = mask;
     for (int i = 0; i < nth; ++i) mm &= mm - 1;
@@ -188,10 +188,11 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + C::STAGES * C::TILE);  // [2]
   uint64_t* q_empty = q_full + 2;                                              // [2]
   uint64_t* s_full = q_full + 4;                                               // [2]
-  uint64_t* p_full = q_full + 6;                                               // [2]
-  uint64_t* o_done = q_full + 8;                                               // [2]
-  uint64_t* drain = q_full + 10;
-  uint64_t* kv_full = q_full + 11;                                             // [STAGES]
+  uint64_t* p_half = q_full + 6;                                               // [2]
+  uint64_t* p_full = q_full + 8;                                               // [2]
+  uint64_t* o_done = q_full + 10;                                              // [2]
+  uint64_t* drain = q_full + 12;
+  uint64_t* kv_full = q_full + 13;                                             // [STAGES]
   uint64_t* kv_empty = kv_full + C::STAGES;                                    // [STAGES]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + C::STAGES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -202,6 +203,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
     }
@@ -228,7 +230,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   griddep_launch_dependents();
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     PackedSched sched(p);
     PackedItem it;
     if (warp == 8) {
@@ -238,7 +240,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       bool ok = true;
       int q_pend[2] = {0, 0};  // Q loads issued
       auto load = [&](const CUtensorMap* map, int col, int row) {
-        ok = ok && mbar_wait(&kv_empty[stage], (use & 1u) ^ 1u, abort_flag, kTagPacked, 21);
+        ok = ok && mbar_wait_hot(&kv_empty[stage], (use & 1u) ^ 1u, abort_flag, kTagPacked, 21);
         if (!ok) return;
         if (lane == 0) {
           mbar_expect_tx(&kv_full[stage], C::TILE);
@@ -258,7 +260,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (it.n[t] == 0 || !ok) continue;
-          ok = mbar_wait(&q_empty[t], (q_pend[t] & 1) ^ 1, abort_flag, kTagPacked, 22);
+          ok = mbar_wait_hot(&q_empty[t], (q_pend[t] & 1) ^ 1, abort_flag, kTagPacked, 22);
           if (ok && lane == 0) {
             mbar_expect_tx(&q_full[t], C::TILE);
 #pragma unroll
@@ -282,91 +284,106 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       }
     } else if (warp == 9) {
       // ---- MMA ----
-      int ks = 0, vs = 0;      // next K and V tile, counted in ring loads (K even, V odd)
+      // Step by step, tile by tile: P V of the step before (the last step of the
+      // item before, at an item's first step), then S of this step.
+      const uint32_t smem_q = smem_u32(smem), ring_u = smem_u32(ring);
+      int n_k = 0;             // steps begun: K is ring load 2 n_k, V is 2 n_k + 1
       int q_use[2] = {0, 0}, p_use[2] = {0, 0};
       bool ok = true;
+      bool pv[2] = {false, false}, more[2] = {false, false};  // P V to do; it adds to O
+      int valid = 0;           // keys of the step before that lie inside the sequence
       auto full = [&](int i, int site) {
-        return mbar_wait(&kv_full[i % C::STAGES], static_cast<uint32_t>(i / C::STAGES) & 1u, abort_flag, kTagPacked, site);
+        return mbar_wait_hot(&kv_full[i % C::STAGES], static_cast<uint32_t>(i / C::STAGES) & 1u, abort_flag, kTagPacked,
+                         site);
+      };
+      // V of the step before has arrived; zero its rows behind the end up to a multiple of 16
+      auto v_ready = [&](int vt) {
+        if (!full(vt, 32)) return false;
+        if (valid & 15) {
+          const int n16 = (16 - (valid & 15)) * (D / 8);
+          for (int i = lane; i < n16; i += 32) {
+            const int r = valid + i / (D / 8), c = i % (D / 8);
+            *reinterpret_cast<uint4*>(ring + (vt % C::STAGES) * C::TILE + (c >> 3) * C::BLOCK + r * 128 +
+                                      (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_shared();
+          __syncwarp();
+        }
+        return true;
+      };
+      auto issue_pv = [&](int t, int vt) {
+        if (!mbar_wait_hot(&p_full[t], static_cast<uint32_t>(p_use[t]++) & 1u, abort_flag, kTagPacked, 33)) return false;
+        tc_fence_after();
+        const int k16 = (valid + 15) / 16;
+        if (elect_one()) {
+          const uint64_t vd = sw128_mnmajor_desc(ring_u + (vt % C::STAGES) * C::TILE, C::BLOCK);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)  // 16 keys: 2048 bytes further
+            if (kk < k16)
+              mma_bf16_ts(tmem + C::O_COL(t), tmem + C::S_COL(t) + kk * 8, vd + kk * 128, C::IDESC_O,
+                          kk > 0 || more[t] ? 1u : 0u);
+          tc_commit(&o_done[t]);
+        }
+        __syncwarp();
+        return true;
       };
       while (ok && sched.next(it)) {
         const int steps = max(it.n[0], it.n[1]);
-        // S of step j and P V of step j + 1 alternate; one pass more than steps
-        for (int j = steps - 1; j >= -1 && ok && steps > 0; --j) {
-          const int kt = 2 * ks, vt = 2 * vs + 1;
-          const bool pv = j + 1 < steps;
-          int valid = 128;  // keys of step j + 1 inside the sequence
-          if (j >= 0) ok = full(kt, 31);
-          if (pv && ok) {
-            ok = full(vt, 32);
-            valid = min(128, it.lk - (j + 1) * 128);
-            if (ok && (valid & 15)) {
-              // zero the rows behind the end up to the next multiple of 16
-              const int r0 = valid, n16 = (16 - (valid & 15)) * (D / 8);
-              for (int i = lane; i < n16; i += 32) {
-                const int r = r0 + i / (D / 8), c = i % (D / 8);
-                *reinterpret_cast<uint4*>(ring + (vt % C::STAGES) * C::TILE + (c >> 3) * C::BLOCK + r * 128 +
-                                          (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
-              }
-              fence_async_shared();
-              __syncwarp();
-            }
-          }
+        for (int j = steps - 1; j >= 0 && ok; --j) {
+          const int kt = 2 * n_k, vt = kt - 1;
+          const bool any = pv[0] || pv[1];
+          if (any) ok = v_ready(vt);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (!ok) break;
-            if (pv && j + 1 < it.n[t]) {
-              ok = mbar_wait(&p_full[t], static_cast<uint32_t>(p_use[t]++) & 1u, abort_flag, kTagPacked, 33);
-              if (!ok) break;
+            if (ok && pv[t]) ok = issue_pv(t, vt);
+            if (t == 0 && ok) ok = full(kt, 31);
+            const bool s = j < it.n[t];
+            if (ok && s) {
+              if (j == it.n[t] - 1)
+                ok = mbar_wait_hot(&q_full[t], static_cast<uint32_t>(q_use[t]++) & 1u, abort_flag, kTagPacked, 35);
               tc_fence_after();
-              if (lane == 0) {
-                const uint32_t va = smem_u32(ring + (vt % C::STAGES) * C::TILE);
-                const int k16 = (valid + 15) / 16;
-                for (int kk = 0; kk < k16; ++kk)
-                  mma_bf16_ts(tmem + C::O_COL(t), tmem + C::S_COL(t) + kk * 8,
-                              sw128_mnmajor_desc(va + kk * 2048, C::BLOCK), C::IDESC_O,
-                              (j + 2 < it.n[t] || kk > 0) ? 1u : 0u);
-                tc_commit(&o_done[t]);
-              }
-              __syncwarp();
-            }
-            if (j >= 0 && j < it.n[t]) {
-              if (j == it.n[t] - 1) {
-                ok = mbar_wait(&q_full[t], static_cast<uint32_t>(q_use[t]++) & 1u, abort_flag, kTagPacked, 34);
-                if (!ok) break;
-              }
-              tc_fence_after();
-              if (lane == 0) {
-                const uint32_t qa = smem_u32(smem + t * C::TILE), ka = smem_u32(ring + (kt % C::STAGES) * C::TILE);
+              if (ok && elect_one()) {
+                const uint64_t qd = sw128_kmajor_desc(smem_q + t * C::TILE);
+                const uint64_t kd = sw128_kmajor_desc(ring_u + (kt % C::STAGES) * C::TILE);
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                  for (int kk = 0; kk < 4; ++kk)
-                    mma_bf16(tmem + C::S_COL(t), sw128_kmajor_desc(qa + b * C::BLOCK + kk * 32),
-                             sw128_kmajor_desc(ka + b * C::BLOCK + kk * 32), C::IDESC_S, (b | kk) != 0 ? 1u : 0u);
+                  for (int kk = 0; kk < 4; ++kk)  // 16 columns: 32 bytes further
+                    mma_bf16(tmem + C::S_COL(t), qd + b * (C::BLOCK / 16) + kk * 2, kd + b * (C::BLOCK / 16) + kk * 2,
+                             C::IDESC_S, (b | kk) != 0 ? 1u : 0u);
                 tc_commit(&s_full[t]);
                 if (j == 0) tc_commit(&q_empty[t]);
               }
               __syncwarp();
             }
+            pv[t] = s;
+            more[t] = j + 1 < it.n[t];
           }
           if (!ok) break;
-          if (lane == 0) {
-            if (j >= 0) tc_commit(&kv_empty[kt % C::STAGES]);
-            if (pv) tc_commit(&kv_empty[vt % C::STAGES]);
+          if (elect_one()) {
+            tc_commit(&kv_empty[kt % C::STAGES]);
+            if (any) tc_commit(&kv_empty[vt % C::STAGES]);
           }
           __syncwarp();
-          if (j >= 0) ++ks;
-          if (pv) ++vs;
+          valid = min(128, it.lk - j * 128);
+          ++n_k;
         }
       }
-      if (lane == 0) {  // every product and every arrival of its commits has happened before the CTA exits
+      if (ok && n_k > 0) {
+        const int vt = 2 * n_k - 1;
+        ok = v_ready(vt);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && pv[t]) ok = issue_pv(t, vt);
+      }
+      if (elect_one()) {  // every product and every arrival of its commits has happened before the CTA exits
         tc_commit(drain);
         mbar_wait_drain(drain, 0);
       }
       __syncwarp();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     PackedSched sched(p);
     PackedItem it;
     // ---- softmax and epilogue: tile t, one row per thread ----
@@ -382,36 +399,43 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       // last visible key of this row
       const int limit = min(it.lk - 1, p.causal ? token + it.lk - it.lq : it.lk - 1);
       const int first_limit = min(it.lk - 1, p.causal ? m + it.lk - it.lq : it.lk - 1);
-      float m_use = -INFINITY, sum = 0.f;
+      float m_use = -INFINITY;
+      float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       for (int j = steps - 1; j >= 0; --j) {
-        ok = mbar_wait(&s_full[t], n_s & 1u, abort_flag, kTagPacked, 41);
+        ok = mbar_wait_hot(&s_full[t], n_s & 1u, abort_flag, kTagPacked, 41);
         if (!ok) break;
         tc_fence_after();
         uint32_t r[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + 32 * c, r[c]);
+        tmem_ld_32x32b_x32(t_s, r[0]);
+        tmem_ld_32x32b_x32(t_s + 32, r[1]);
         tmem_ld_wait();
-        if (j * 128 + 127 > first_limit) {
-          const int lim = limit - j * 128;
+        tmem_ld_32x32b_x32(t_s + 64, r[2]);
+        tmem_ld_32x32b_x32(t_s + 96, r[3]);
+        const bool cut = j * 128 + 127 > first_limit;
+        const int lim = limit - j * 128;
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // independent chains
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c) {
+          if (c == 2) tmem_ld_wait();
+          if (cut) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i > lim) r[c][i] = 0xff800000u;  // -inf
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            mx4[(i >> 1) & 3] = fmaxf(mx4[(i >> 1) & 3], fmaxf(__uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1])));
         }
-        float mx = __uint_as_float(r[0][0]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[c][i]));
         // powers of two of scaled scores; the maximum in use follows when some row of the warp outgrew it
-        mx = fmaxf(mx * p.scale_log2e, m_use);
+        const float mx =
+            fmaxf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2e, m_use);
         if (__any_sync(0xffffffffu, mx > m_use + 8.f)) {
           const float f = mx == -INFINITY ? 1.f : ex2_approx(m_use - mx);
           m_use = mx;
-          sum *= f;
+          sum2[0] = __fmul2_rn(sum2[0], make_float2(f, f));
+          sum2[1] = __fmul2_rn(sum2[1], make_float2(f, f));
           if (j != steps - 1) {
-            ok = mbar_wait(&o_done[t], (n_s - 1) & 1u, abort_flag, kTagPacked, 42);
+            ok = mbar_wait_hot(&o_done[t], (n_s - 1) & 1u, abort_flag, kTagPacked, 42);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -426,19 +450,23 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           }
         }
         const float off = m_use == -INFINITY ? 0.f : -m_use;
+        const float2 off2 = make_float2(off, off), scale2 = make_float2(p.scale_log2e, p.scale_log2e);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t pk[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int c = 2 * h + (i >> 4), k = (2 * i) & 31;
-            const float e0 = ex2_approx(fmaf(__uint_as_float(r[c][k]), p.scale_log2e, off));
-            const float e1 = ex2_approx(fmaf(__uint_as_float(r[c][k + 1]), p.scale_log2e, off));
-            sum += e0 + e1;
-            const __nv_bfloat162 b = __floats2bfloat162_rn(e0, e1);
-            pk[i] = *reinterpret_cast<const uint32_t*>(&b);
+          for (int c = 2 * h; c < 2 * h + 2; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 x = __ffma2_rn(
+                  make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), scale2, off2);
+              const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              sum2[i & 1] = __fadd2_rn(sum2[i & 1], e);
+              const __nv_bfloat162 b = __floats2bfloat162_rn(e.x, e.y);
+              pk[i] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            tmem_st_32x32b_x16(t_s + 16 * c, pk);
           }
-          tmem_st_32x32b_x32(t_s + 32 * h, pk);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -447,6 +475,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         ++n_s;
       }
       if (!ok) break;
+      const float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
       const bool live = token < it.lq;
       const long long grow = it.q0 + token;
       __nv_bfloat16* dst = p.out + grow * p.ldo + head * D;
@@ -458,7 +487,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0u, 0u, 0u, 0u);
         continue;
       }
-      ok = mbar_wait(&o_done[t], (n_s - 1) & 1u, abort_flag, kTagPacked, 43);
+      ok = mbar_wait_hot(&o_done[t], (n_s - 1) & 1u, abort_flag, kTagPacked, 43);
       if (!ok) break;
       tc_fence_after();
       const float inv = sum > 0.f ? 1.f / sum : 0.f;

@@ -93,6 +93,7 @@ static int launch_packed(const void* q, long long ldq, const void* k, long long 
   // sequences are bounded by their number
   const long long rows = p.pair_heads ? 128 : 256;
   const long long items = (p.total_q / rows + p.n_seq) * (p.pair_heads ? p.heads / 2 : p.heads);
+  if (items > 0x7fff0000ll) return QI_B200_ETOOBIG;  // the kernel counts items in 32 bits
   const int grid = static_cast<int>(std::min<long long>(num_sms, std::max(1ll, items)));
   return launched(launch_pdl(k_attn_packed<D>, dim3(grid), dim3(C::THREADS), C::SMEM, stream, 1, tq, tk, tv, p));
 }

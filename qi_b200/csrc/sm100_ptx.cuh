@@ -45,6 +45,16 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
   return t;
 }
 
+// True in one thread of the (converged) warp, always the same one.  A branch
+// on it lets the compiler keep the operands of tensor-core instructions in
+// uniform registers, which a branch on the lane number does not.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(ok));
+  return ok != 0;
+}
+
 // Load with acquire semantics at GPU scope (a counter other CTAs release to).
 __device__ __forceinline__ unsigned int ld_acquire_gpu(const unsigned int* p) {
   unsigned int v;
@@ -114,6 +124,17 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
       return false;
     }
   }
+}
+
+// mbar_wait for handovers on a kernel's critical path: it looks at the timer
+// and the abort flag only after many tries, because reading %globaltimer takes
+// long enough to delay the handover.
+__device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                              unsigned int tag, unsigned int site) {
+#pragma unroll 1
+  for (int i = 0; i < 512; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, abort_flag, tag, site);
 }
 
 // Wait used only while draining after an abort: shorter limit, no new error.
