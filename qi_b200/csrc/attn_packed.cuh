@@ -20,13 +20,26 @@
 // maximum rarely grows.
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of tile 0 and 1, warp 8 TMA,
-// warp 9 MMA (10 and 11 fill up their warpgroup).  A softmax thread holds a
-// whole row of S, so the softmax warpgroups take 216 registers a thread and
-// the third leaves them all but 72 (of 168 at launch: 256 x 216 + 128 x 72 =
-// 64,512, all of them).  CTAs are persistent; each takes every gridDim.x-th item, longest
-// items first, the direction alternating from round to round.  The order is a
-// function of cu_q alone: level L (the L-th query block of every sequence that
-// has one) from the last to the first, so no list of items is stored.
+// warp 9 MMA, warp 10 the list of items (11 fills up the warpgroup).  A softmax
+// thread holds a whole row of S, so the softmax warpgroups take 208 registers a
+// thread and the third leaves them all but 88 (of 168 at launch: 256 x 208 +
+// 128 x 88 = 64,512, all of them).  CTAs are persistent; each takes every
+// gridDim.x-th item, longest items first, the direction alternating from round
+// to round.  The order is a function of cu_q alone: level L (the L-th query
+// block of every sequence that has one) from the last to the first; warp 10
+// walks it and hands the items over in shared memory, four in flight.
+//
+// What bounds it: the chain of one tile, softmax (about 2,250 clocks, 1,024 of
+// them exponentials) then P V and S (1,300 clocks, 1,024 of them products),
+// 3,750 clocks per 128-key step where the products of both tiles take 2,048.
+// Measured on the way (16384 tokens, 24 / 8 heads of 128, causal, us): products
+// issued by lane 0 with 64-bit descriptors formed on the spot 1,842, by an
+// elected thread 1,645, item list in a warp of its own and descriptors as
+// constants to a base 1,371, all MMA operands warp-uniform 1,330.  Two threads
+// per row (16 softmax warps) 1,433; half of P handed over early 1,359; 64-key
+// steps with S double-buffered 1,457 (the products read shared memory at its
+// full rate then, and every barrier waits behind them); a quarter of the
+// exponentials as polynomials on the FP32 pipe 1,365.
 //
 // Rows behind a sequence's end belong to its neighbour: scores of such keys
 // are replaced (not added to), the V rows of the last 16-key step behind the
@@ -39,6 +52,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "attn_short.cuh"
 #include "launch_count.cuh"
@@ -61,17 +75,44 @@ struct PackedParams {
   float* lse;        // [total_q, heads] or nullptr
 };
 
-// Descriptor of an operand whose rows are the K extent (MN-major): rows of 64
-// elements (128 B, 128-byte swizzle), 8-row groups 1024 B apart, blocks of 64
-// MN elements `lead` bytes apart.
-__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr, uint32_t lead) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>(lead >> 4) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
+// Shared-memory descriptors as two words.  The high word is a constant (8-row
+// groups 1024 B apart, version 1, 128-byte swizzle); the low word holds the
+// address / 16 and the leading offset / 16: unused (1) for K-major operands;
+// for V, whose rows are the K extent (MN-major), the distance of its blocks of
+// 64 columns.  Products of a tile differ in the low word by constants.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr, uint32_t lead) {
+  return ((smem_addr & 0x3FFFFu) >> 4) | ((lead >> 4) << 16);
+}
+// A value the compiler cannot see through: sums with it are formed where they
+// are used.  Without it the 50 descriptors of the unrolled steps are all formed
+// ahead of the loop and kept on the stack, whose loads delay every product.
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+__device__ __forceinline__ void tc_commit_if(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_bf16_lo(uint32_t leader, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi), "r"(leader));
+}
+__device__ __forceinline__ void mma_bf16_ts_lo(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo,
+                                               uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi), "r"(leader));
 }
 
 __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -90,9 +131,10 @@ template <int D>
 struct PackedCfg {
   static constexpr int TILE = 128 * D * 2;       // bytes of a 128-row operand tile (D / 64 swizzled blocks)
   static constexpr int BLOCK = 128 * 128;        // bytes of one 64-column block
-  static constexpr int STAGES = D == 128 ? 4 : 8;
+  static constexpr int STAGES = 4;               // K and V of two steps
   static constexpr int THREADS = 384;
-  static constexpr int SMEM = (2 + STAGES) * TILE + 1024 + 256;
+  static constexpr int STAGING = 8 * 4096;       // 32 rows x 128 B of output per softmax warp
+  static constexpr int SMEM = (2 + STAGES) * TILE + STAGING + 1024 + 512;
   static constexpr int TMEM_COLS = 512;
   __host__ __device__ static constexpr uint32_t S_COL(int t) { return t * 128; }
   __host__ __device__ static constexpr uint32_t O_COL(int t) { return 256 + t * D; }
@@ -100,81 +142,74 @@ struct PackedCfg {
   static constexpr uint32_t IDESC_O = make_idesc(kDF32, kFmtBF16, kFmtBF16, 128, D) | (1u << 16);  // B is MN-major
 };
 
-// One work item.
+// One work item, as the scheduling warp puts it into shared memory.
 struct PackedItem {
   int q0, lq, k0, lk;  // first rows and lengths of the sequence
   int m[2], head[2];   // first token (inside the sequence) and head of the two tiles
   int n[2];            // 128-key steps of the two tiles (0: nothing visible, or no rows)
+  int last;            // 1: there is no item, the CTA is done
+  int pad;
 };
+constexpr int kPackedItems = 4;  // items in flight
 
-// The items of one CTA in order; every warp walks the same sequence.
-struct PackedSched {
-  const PackedParams& p;
-  int lane, rows_per_item, heads_items;
-  int level, chunk;
-  int base;            // items before the current (level, chunk)
-  int round;
-  unsigned mask;       // active sequences of the chunk
-  int blocks0;         // query blocks of sequence `lane` (chunk 0)
+// Rows of sequence b, clamped to the tensor (bad prefix sums read and write inside it).
+__device__ __forceinline__ void packed_span(const int* cu, int b, int total, int& first, int& len) {
+  first = min(max(cu[b], 0), total);
+  len = min(max(cu[b + 1], first), total) - first;
+}
 
-  __device__ __forceinline__ int seq_blocks(int b) const {
+// The items of this CTA, longest first, one after another into `out` (the whole warp calls it).
+template <class Put>
+__device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) {
+  const int lane = threadIdx.x & 31;
+  const int rows_per_item = p.pair_heads ? 128 : 256;
+  const int heads_items = p.pair_heads ? p.heads / 2 : p.heads;
+  auto blocks = [&](int b) {
     if (b >= p.n_seq) return 0;
-    int q0, lq;
-    span(p.cu_q, b, p.total_q, q0, lq);
-    return (lq + rows_per_item - 1) / rows_per_item;
-  }
-  // rows of sequence b, clamped to the tensor (bad prefix sums read and write inside it)
-  __device__ __forceinline__ static void span(const int* cu, int b, int total, int& first, int& len) {
-    first = min(max(cu[b], 0), total);
-    len = min(max(cu[b + 1], first), total) - first;
-  }
-  __device__ __forceinline__ PackedSched(const PackedParams& pp) : p(pp) {
-    lane = threadIdx.x & 31;
-    rows_per_item = p.pair_heads ? 128 : 256;
-    heads_items = p.pair_heads ? p.heads / 2 : p.heads;
-    int most = 0;
-    for (int b = lane; b < p.n_seq; b += 32) most = max(most, seq_blocks(b));
+    int first, len;
+    packed_span(p.cu_q, b, p.total_q, first, len);
+    return (len + rows_per_item - 1) / rows_per_item;
+  };
+  int most = 0;
+  for (int b = lane; b < p.n_seq; b += 32) most = max(most, blocks(b));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    blocks0 = seq_blocks(lane);
-    level = most - 1;
-    chunk = 0;
-    base = 0;
-    round = 0;
-    mask = __ballot_sync(0xffffffffu, blocks0 > level);
-  }
-  __device__ __forceinline__ bool next(PackedItem& it) {
-    const int G = gridDim.x;
-    const int target = round * G + ((round & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
-    if (level < 0) return false;
-    while (target >= base + __popc(mask) * heads_items) {
-      base += __popc(mask) * heads_items;
-      chunk += 32;
-      if (chunk >= p.n_seq) {
-        chunk = 0;
-        if (--level < 0) return false;
+  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const int blocks0 = blocks(lane);
+  const int G = gridDim.x, me = blockIdx.x;
+  int base = 0, round = 0;  // items before this (level, chunk); rounds of G items begun
+  for (int level = most - 1; level >= 0; --level) {
+    for (int chunk = 0; chunk < p.n_seq; chunk += 32) {
+      unsigned active = __ballot_sync(0xffffffffu, (chunk == 0 ? blocks0 : blocks(chunk + lane)) > level);
+      const int n = __popc(active) * heads_items;
+      while (true) {
+        const int idx = round * G + ((round & 1) ? G - 1 - me : me) - base;
+        if (idx >= n) break;
+        ++round;
+        const int nth = idx / heads_items, hi = idx - nth * heads_items;
+        unsigned mm = active;
+        for (int i = 0; i < nth; ++i) mm &= mm - 1;
+        const int b = chunk + __ffs(mm) - 1;
+        PackedItem it;
+        packed_span(p.cu_q, b, p.total_q, it.q0, it.lq);
+        packed_span(p.cu_k, b, p.total_k, it.k0, it.lk);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          it.head[t] = p.pair_heads ? 2 * hi + t : hi;
+          it.m[t] = level * rows_per_item + (p.pair_heads ? 0 : 128 * t);
+          const int rows = min(128, it.lq - it.m[t]);
+          const int visible = p.causal ? min(it.lk, it.m[t] + rows + it.lk - it.lq) : it.lk;
+          it.n[t] = rows > 0 && visible > 0 ? (visible + 127) / 128 : 0;
+        }
+        it.last = it.pad = 0;
+        if (!put(it)) return;
       }
-      mask = __ballot_sync(0xffffffffu, (chunk == 0 ? blocks0 : seq_blocks(chunk + lane)) > level);
+      base += n;
     }
-    ++round;
-    const int idx = target - base;
-    const int nth = idx / heads_items, hi = idx - nth * heads_items;
-    unsigned mm = mask;
-    for (int i = 0; i < nth; ++i) mm &= mm - 1;
-    const int b = chunk + __ffs(mm) - 1;
-    span(p.cu_q, b, p.total_q, it.q0, it.lq);
-    span(p.cu_k, b, p.total_k, it.k0, it.lk);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      it.head[t] = p.pair_heads ? 2 * hi + t : hi;
-      it.m[t] = level * rows_per_item + (p.pair_heads ? 0 : 128 * t);
-      const int rows = min(128, it.lq - it.m[t]);
-      const int visible = p.causal ? min(it.lk, it.m[t] + rows + it.lk - it.lq) : it.lk;
-      it.n[t] = rows > 0 && visible > 0 ? (visible + 127) / 128 : 0;
-    }
-    return true;
   }
-};
+  PackedItem end = {};
+  end.last = 1;
+  put(end);
+}
 
 template <int D>
 __global__ void __launch_bounds__(384, 1)
@@ -185,16 +220,19 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   extern __shared__ uint8_t packed_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(packed_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + 2 * C::TILE;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + C::STAGES * C::TILE);  // [2]
+  uint8_t* staging = ring + C::STAGES * C::TILE;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(staging + C::STAGING);        // [2]
   uint64_t* q_empty = q_full + 2;                                              // [2]
   uint64_t* s_full = q_full + 4;                                               // [2]
-  uint64_t* p_half = q_full + 6;                                               // [2]
-  uint64_t* p_full = q_full + 8;                                               // [2]
-  uint64_t* o_done = q_full + 10;                                              // [2]
-  uint64_t* drain = q_full + 12;
-  uint64_t* kv_full = q_full + 13;                                             // [STAGES]
+  uint64_t* p_full = q_full + 6;                                               // [2]
+  uint64_t* o_done = q_full + 8;                                               // [2]
+  uint64_t* drain = q_full + 10;
+  uint64_t* kv_full = q_full + 11;                                             // [STAGES]
   uint64_t* kv_empty = kv_full + C::STAGES;                                    // [STAGES]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + C::STAGES);
+  uint64_t* it_full = kv_empty + C::STAGES;                                    // [kPackedItems]
+  uint64_t* it_empty = it_full + kPackedItems;                                 // [kPackedItems]
+  PackedItem* items = reinterpret_cast<PackedItem*>(it_empty + kPackedItems);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kPackedItems);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -203,7 +241,6 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
     }
@@ -211,6 +248,10 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
+    }
+    for (int i = 0; i < kPackedItems; ++i) {
+      mbar_init(&it_full[i], 1);
+      mbar_init(&it_empty[i], 10);  // the softmax warps, TMA and MMA
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -225,15 +266,40 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   griddep_wait();
   griddep_launch_dependents();
 
+  // the next item (nullptr: none, or the CTA gives up), and its release
+  uint32_t n_it = 0;
+  auto next_item = [&]() -> const PackedItem* {
+    if (!mbar_wait_hot(&it_full[n_it % kPackedItems], (n_it / kPackedItems) & 1u, abort_flag, kTagPacked, 11))
+      return nullptr;
+    const PackedItem* it = &items[n_it % kPackedItems];
+    return it->last ? nullptr : it;
+  };
+  auto release_item = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&it_empty[n_it % kPackedItems]);
+    ++n_it;
+  };
+
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    PackedSched sched(p);
-    PackedItem it;
-    if (warp == 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 10) {
+      // ---- items ----
+      packed_schedule(p, [&](const PackedItem& it) {
+        const int i = n_it % kPackedItems;
+        if (!mbar_wait_hot(&it_empty[i], ((n_it / kPackedItems) & 1u) ^ 1u, abort_flag, kTagPacked, 12)) return false;
+        if (lane == 0) {
+          items[i] = it;
+          mbar_arrive(&it_full[i]);
+        }
+        __syncwarp();
+        ++n_it;
+        return true;
+      });
+    } else if (warp == 8) {
       // ---- TMA ----
       int stage = 0, issued = 0;
       uint32_t use = 0;  // times the ring has been gone round
@@ -254,26 +320,30 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           ++use;
         }
       };
-      while (ok && sched.next(it)) {
-        const int steps = max(it.n[0], it.n[1]);
-        if (steps == 0) continue;
+      while (const PackedItem* it = next_item()) {
+        const int steps = max(it->n[0], it->n[1]);
+        const int q0 = it->q0, k0 = it->k0, col = it->head[0] / p.group * D;
+        if (steps > 0) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (it.n[t] == 0 || !ok) continue;
-          ok = mbar_wait_hot(&q_empty[t], (q_pend[t] & 1) ^ 1, abort_flag, kTagPacked, 22);
-          if (ok && lane == 0) {
-            mbar_expect_tx(&q_full[t], C::TILE);
+          for (int t = 0; t < 2; ++t) {
+            if (it->n[t] == 0 || !ok) continue;
+            ok = mbar_wait_hot(&q_empty[t], (q_pend[t] & 1) ^ 1, abort_flag, kTagPacked, 22);
+            if (ok && lane == 0) {
+              mbar_expect_tx(&q_full[t], C::TILE);
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-              tma_load_2d(smem + t * C::TILE + b * C::BLOCK, &tmQ, &q_full[t], it.head[t] * D + b * 64, it.q0 + it.m[t]);
+              for (int b = 0; b < NB; ++b)
+                tma_load_2d(smem + t * C::TILE + b * C::BLOCK, &tmQ, &q_full[t], it->head[t] * D + b * 64,
+                            q0 + it->m[t]);
+            }
+            if (ok) ++q_pend[t];
           }
-          if (ok) ++q_pend[t];
         }
-        const int col = it.head[0] / p.group * D;
+        release_item();
         for (int j = steps - 1; j >= 0 && ok; --j) {
-          load(&tmK, col, it.k0 + j * 128);
-          load(&tmV, col, it.k0 + j * 128);
+          load(&tmK, col, k0 + j * 128);
+          load(&tmV, col, k0 + j * 128);
         }
+        if (!ok) break;
       }
       if (*abort_flag) {
         // let the copies in flight land before the CTA exits
@@ -284,121 +354,139 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       }
     } else if (warp == 9) {
       // ---- MMA ----
-      // Step by step, tile by tile: P V of the step before (the last step of the
-      // item before, at an item's first step), then S of this step.
-      const uint32_t smem_q = smem_u32(smem), ring_u = smem_u32(ring);
+      // The whole warp runs this with warp-uniform values (counts are broadcast,
+      // waits end in a vote), one elected thread issues: operands then stay in
+      // uniform registers.  Step by step, tile by tile: P V of the step before (the
+      // last step of the item before, at an item's first step), then S of this step.
+      const uint32_t q_lo = desc_lo(smem_u32(smem), 16), k_lo = desc_lo(smem_u32(ring), 16);
+      const uint32_t v_lo = desc_lo(smem_u32(ring) + C::TILE, C::BLOCK);
+      const uint32_t leader = elect_one();
       int n_k = 0;             // steps begun: K is ring load 2 n_k, V is 2 n_k + 1
-      int q_use[2] = {0, 0}, p_use[2] = {0, 0};
+      uint32_t q_use0 = 0, q_use1 = 0, p_use0 = 0, p_use1 = 0;
+      bool pv0 = false, pv1 = false;      // P V of the step before to do, per tile
+      uint32_t more0 = 0, more1 = 0;      // it adds to O
+      bool last = false;                  // it is its item's last
+      int valid = 0;                      // keys of the step before that lie inside the sequence
       bool ok = true;
-      bool pv[2] = {false, false}, more[2] = {false, false};  // P V to do; it adds to O
-      int valid = 0;           // keys of the step before that lie inside the sequence
+      auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+        return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag, kTagPacked, site)) != 0;
+      };
       auto full = [&](int i, int site) {
-        return mbar_wait_hot(&kv_full[i % C::STAGES], static_cast<uint32_t>(i / C::STAGES) & 1u, abort_flag, kTagPacked,
-                         site);
+        return wait(&kv_full[i % C::STAGES], static_cast<uint32_t>(i / C::STAGES) & 1u, site);
       };
       // V of the step before has arrived; zero its rows behind the end up to a multiple of 16
-      auto v_ready = [&](int vt) {
+      auto v_ready = [&]() {
+        const int vt = 2 * n_k - 1;
         if (!full(vt, 32)) return false;
         if (valid & 15) {
+          uint8_t* v = ring + (vt % C::STAGES) * C::TILE;
           const int n16 = (16 - (valid & 15)) * (D / 8);
           for (int i = lane; i < n16; i += 32) {
             const int r = valid + i / (D / 8), c = i % (D / 8);
-            *reinterpret_cast<uint4*>(ring + (vt % C::STAGES) * C::TILE + (c >> 3) * C::BLOCK + r * 128 +
-                                      (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(v + (c >> 3) * C::BLOCK + r * 128 + ((c & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
           }
           fence_async_shared();
           __syncwarp();
         }
         return true;
       };
-      auto issue_pv = [&](int t, int vt) {
-        if (!mbar_wait_hot(&p_full[t], static_cast<uint32_t>(p_use[t]++) & 1u, abort_flag, kTagPacked, 33)) return false;
+      // V of step n_k - 1
+      auto issue_pv = [&](auto tile, uint32_t& use, uint32_t more) {
+        constexpr int t = decltype(tile)::value;
+        if (!wait(&p_full[t], use & 1u, 33)) return false;
+        ++use;
         tc_fence_after();
-        const int k16 = (valid + 15) / 16;
-        if (elect_one()) {
-          const uint64_t vd = sw128_mnmajor_desc(ring_u + (vt % C::STAGES) * C::TILE, C::BLOCK);
+        const uint32_t vd = v_lo + ((n_k - 1) & 1) * (2 * C::TILE / 16);
+        if (valid > 112) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)  // 16 keys: 2048 bytes further
-            if (kk < k16)
-              mma_bf16_ts(tmem + C::O_COL(t), tmem + C::S_COL(t) + kk * 8, vd + kk * 128, C::IDESC_O,
-                          kk > 0 || more[t] ? 1u : 0u);
-          tc_commit(&o_done[t]);
+            mma_bf16_ts_lo(leader, tmem + C::O_COL(t), tmem + C::S_COL(t) + kk * 8, vd + kk * 128, C::IDESC_O,
+                           kk > 0 ? 1u : more);
+        } else {
+          for (int kk = 0; kk * 16 < valid; ++kk)
+            mma_bf16_ts_lo(leader, tmem + C::O_COL(t), tmem + C::S_COL(t) + kk * 8, vd + kk * 128, C::IDESC_O,
+                           kk > 0 ? 1u : more);
         }
-        __syncwarp();
+        if (last) tc_commit_if(leader, &o_done[t]);
         return true;
       };
-      while (ok && sched.next(it)) {
-        const int steps = max(it.n[0], it.n[1]);
-        for (int j = steps - 1; j >= 0 && ok; --j) {
-          const int kt = 2 * n_k, vt = kt - 1;
-          const bool any = pv[0] || pv[1];
-          if (any) ok = v_ready(vt);
+      auto issue_s = [&](auto tile, uint32_t& use, bool first, bool end) {
+        constexpr int t = decltype(tile)::value;
+        if (first) {
+          if (!wait(&q_full[t], use & 1u, 35)) return false;
+          ++use;
+        }
+        tc_fence_after();
+        const uint32_t qd = q_lo + t * (C::TILE / 16), kd = k_lo + (n_k & 1) * (2 * C::TILE / 16);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (ok && pv[t]) ok = issue_pv(t, vt);
-            if (t == 0 && ok) ok = full(kt, 31);
-            const bool s = j < it.n[t];
-            if (ok && s) {
-              if (j == it.n[t] - 1)
-                ok = mbar_wait_hot(&q_full[t], static_cast<uint32_t>(q_use[t]++) & 1u, abort_flag, kTagPacked, 35);
-              tc_fence_after();
-              if (ok && elect_one()) {
-                const uint64_t qd = sw128_kmajor_desc(smem_q + t * C::TILE);
-                const uint64_t kd = sw128_kmajor_desc(ring_u + (kt % C::STAGES) * C::TILE);
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                  for (int kk = 0; kk < 4; ++kk)  // 16 columns: 32 bytes further
-                    mma_bf16(tmem + C::S_COL(t), qd + b * (C::BLOCK / 16) + kk * 2, kd + b * (C::BLOCK / 16) + kk * 2,
-                             C::IDESC_S, (b | kk) != 0 ? 1u : 0u);
-                tc_commit(&s_full[t]);
-                if (j == 0) tc_commit(&q_empty[t]);
-              }
-              __syncwarp();
-            }
-            pv[t] = s;
-            more[t] = j + 1 < it.n[t];
-          }
-          if (!ok) break;
-          if (elect_one()) {
-            tc_commit(&kv_empty[kt % C::STAGES]);
-            if (any) tc_commit(&kv_empty[vt % C::STAGES]);
-          }
-          __syncwarp();
-          valid = min(128, it.lk - j * 128);
+          for (int kk = 0; kk < 4; ++kk)  // 16 columns: 32 bytes further
+            mma_bf16_lo(leader, tmem + C::S_COL(t), qd + b * (C::BLOCK / 16) + kk * 2,
+                        kd + b * (C::BLOCK / 16) + kk * 2, C::IDESC_S, (b | kk) != 0 ? 1u : 0u);
+        tc_commit_if(leader, &s_full[t]);
+        if (end) tc_commit_if(leader, &q_empty[t]);
+        return true;
+      };
+      using Zero = std::integral_constant<int, 0>;
+      using One = std::integral_constant<int, 1>;
+      auto finish = [&]() {  // P V of the last step, where no S follows
+        if (!pv0 && !pv1) return true;
+        if (!v_ready()) return false;
+        if (pv0 && !issue_pv(Zero(), p_use0, more0)) return false;
+        if (pv1 && !issue_pv(One(), p_use1, more1)) return false;
+        tc_commit_if(leader, &kv_empty[(2 * n_k - 1) % C::STAGES]);
+        pv0 = pv1 = false;
+        return true;
+      };
+      while (const PackedItem* it = next_item()) {
+        const int n0 = __shfl_sync(0xffffffffu, it->n[0], 0), n1 = __shfl_sync(0xffffffffu, it->n[1], 0);
+        const int lk = __shfl_sync(0xffffffffu, it->lk, 0), steps = max(n0, n1);
+        release_item();
+        // an item without keys brings no step, and many of them may follow: the
+        // softmax warps have to get through the item before without one
+        if (steps == 0) ok = finish();
+        for (int j = steps - 1; j >= 0; --j) {
+          const bool any = pv0 || pv1, s0 = j < n0, s1 = j < n1;
+          if (!(ok = !any || v_ready())) break;
+          if (!(ok = full(2 * n_k, 31))) break;
+          if (pv0 && !(ok = issue_pv(Zero(), p_use0, more0))) break;
+          if (s0 && !(ok = issue_s(Zero(), q_use0, j == n0 - 1, j == 0))) break;
+          if (pv1 && !(ok = issue_pv(One(), p_use1, more1))) break;
+          if (s1 && !(ok = issue_s(One(), q_use1, j == n1 - 1, j == 0))) break;
+          tc_commit_if(leader, &kv_empty[(2 * n_k) % C::STAGES]);
+          if (any) tc_commit_if(leader, &kv_empty[(2 * n_k - 1) % C::STAGES]);
+          pv0 = s0, pv1 = s1;
+          more0 = j + 1 < n0, more1 = j + 1 < n1;
+          last = j == 0;
+          valid = min(128, lk - j * 128);
           ++n_k;
         }
+        if (!ok) break;
       }
-      if (ok && n_k > 0) {
-        const int vt = 2 * n_k - 1;
-        ok = v_ready(vt);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (ok && pv[t]) ok = issue_pv(t, vt);
-      }
-      if (elect_one()) {  // every product and every arrival of its commits has happened before the CTA exits
-        tc_commit(drain);
-        mbar_wait_drain(drain, 0);
-      }
+      if (ok) ok = finish();
+      // every product and every arrival of its commits has happened before the CTA exits
+      tc_commit_if(leader, drain);
+      mbar_wait_drain(drain, 0);
       __syncwarp();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    PackedSched sched(p);
-    PackedItem it;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax and epilogue: tile t, one row per thread ----
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_s = t_lane + C::S_COL(t), t_o = t_lane + C::O_COL(t);
-    uint32_t n_s = 0;  // steps done so far (phases of s_full and o_done)
+    uint32_t n_s = 0, n_items = 0;  // steps and items done so far (phases of s_full and o_done)
     bool ok = true;
-    while (ok && sched.next(it)) {
-      const int m = t ? it.m[1] : it.m[0], steps = t ? it.n[1] : it.n[0], head = t ? it.head[1] : it.head[0];
-      const int token = m + row;
-      // last visible key of this row
-      const int limit = min(it.lk - 1, p.causal ? token + it.lk - it.lq : it.lk - 1);
-      const int first_limit = min(it.lk - 1, p.causal ? m + it.lk - it.lq : it.lk - 1);
+    while (const PackedItem* it = next_item()) {
+      const int steps = it->n[t];
+      int limit, first_limit;  // last visible key of this row and of the tile's first row
+      {
+        const int lk = it->lk, m = it->m[t], reach = p.causal ? m + lk - it->lq : lk - 1;
+        first_limit = min(lk - 1, reach);
+        limit = min(lk - 1, p.causal ? reach + row : reach);
+      }
       float m_use = -INFINITY;
       float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       for (int j = steps - 1; j >= 0; --j) {
@@ -426,47 +514,42 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           for (int i = 0; i < 32; i += 2)
             mx4[(i >> 1) & 3] = fmaxf(mx4[(i >> 1) & 3], fmaxf(__uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1])));
         }
+        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
         // powers of two of scaled scores; the maximum in use follows when some row of the warp outgrew it
-        const float mx =
-            fmaxf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2e, m_use);
+        mx = fmaxf(mx * p.scale_log2e, m_use);
         if (__any_sync(0xffffffffu, mx > m_use + 8.f)) {
           const float f = mx == -INFINITY ? 1.f : ex2_approx(m_use - mx);
           m_use = mx;
           sum2[0] = __fmul2_rn(sum2[0], make_float2(f, f));
           sum2[1] = __fmul2_rn(sum2[1], make_float2(f, f));
-          if (j != steps - 1) {
-            ok = mbar_wait_hot(&o_done[t], (n_s - 1) & 1u, abort_flag, kTagPacked, 42);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(t_o + 32 * c, o);
+          if (j != steps - 1) {  // S of this step was multiplied after P V of the step before: O is at rest
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(t_o + 16 * c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st_32x32b_x32(t_o + 32 * c, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st_32x32b_x16(t_o + 16 * c, o);
             }
           }
         }
         const float off = m_use == -INFINITY ? 0.f : -m_use;
         const float2 off2 = make_float2(off, off), scale2 = make_float2(p.scale_log2e, p.scale_log2e);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int c = 0; c < 8; ++c) {
+          uint32_t pk[8];
 #pragma unroll
-          for (int c = 2 * h; c < 2 * h + 2; ++c) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 x = __ffma2_rn(
-                  make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), scale2, off2);
-              const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-              sum2[i & 1] = __fadd2_rn(sum2[i & 1], e);
-              const __nv_bfloat162 b = __floats2bfloat162_rn(e.x, e.y);
-              pk[i] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            tmem_st_32x32b_x16(t_s + 16 * c, pk);
+          for (int i = 0; i < 8; ++i) {
+            const int k = (c & 1) * 16 + 2 * i;
+            const float2 x = __ffma2_rn(
+                make_float2(__uint_as_float(r[c >> 1][k]), __uint_as_float(r[c >> 1][k + 1])), scale2, off2);
+            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            sum2[i & 1] = __fadd2_rn(sum2[i & 1], e);
+            const __nv_bfloat162 b = __floats2bfloat162_rn(e.x, e.y);
+            pk[i] = *reinterpret_cast<const uint32_t*>(&b);
           }
+          tmem_st_32x32b_x8(t_s + 8 * c, pk);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -475,38 +558,56 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         ++n_s;
       }
       if (!ok) break;
-      const float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-      const bool live = token < it.lq;
-      const long long grow = it.q0 + token;
-      __nv_bfloat16* dst = p.out + grow * p.ldo + head * D;
-      if (live && p.lse != nullptr)
-        p.lse[grow * p.heads + head] = sum > 0.f ? (m_use + log2f(sum)) * 0.69314718055994531f : -INFINITY;
-      if (steps == 0) {
-        if (live)
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0u, 0u, 0u, 0u);
-        continue;
+      const int head = it->head[t], rows = min(128, it->lq - it->m[t]) - (warp & 3) * 32;  // rows of this warp's 32
+      const long long first = it->q0 + it->m[t] + (warp & 3) * 32;
+      __nv_bfloat16* dst = p.out + first * p.ldo + head * D;
+      float* lse = p.lse != nullptr && lane < rows ? p.lse + (first + lane) * p.heads + head : nullptr;
+      float inv = 0.f;  // a row that saw no key gives zeros
+      if (steps > 0) {
+        ok = mbar_wait_hot(&o_done[t], n_items++ & 1u, abort_flag, kTagPacked, 43);
+        if (!ok) break;
+        tc_fence_after();
+        const float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+        if (m_use > -INFINITY) inv = 1.f / sum;
+        if (lse != nullptr) *lse = m_use > -INFINITY ? (m_use + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+      } else if (lse != nullptr) {
+        *lse = -INFINITY;
       }
-      ok = mbar_wait_hot(&o_done[t], (n_s - 1) & 1u, abort_flag, kTagPacked, 43);
-      if (!ok) break;
-      tc_fence_after();
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      // 64 columns at a time through shared memory (chunks permuted by the row, so
+      // that neither side has bank conflicts), so that a store covers whole lines;
+      // a row per thread would touch 32 lines with each
+      uint8_t* box = staging + warp * 4096;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(t_o + 32 * c, o);
-        tmem_ld_wait();
-        if (live) {
+      for (int c = 0; c < D / 64; ++c) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32];
+          if (steps > 0) {
+            tmem_ld_32x32b_x32(t_o + 64 * c + 32 * h, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * i + e]) * inv;
-            reinterpret_cast<uint4*>(dst)[c * 4 + i] = pack8(f);
+            *reinterpret_cast<uint4*>(box + lane * 128 + (((4 * h + i) ^ (lane & 7)) << 4)) = pack8(f);
           }
         }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + (lane >> 3);
+          const uint4 v = *reinterpret_cast<const uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          if (r < rows) *reinterpret_cast<uint4*>(dst + r * p.ldo + 64 * c + (lane & 7) * 8) = v;
+        }
+        __syncwarp();
       }
       tc_fence_before();
+      release_item();
     }
   }
   tc_fence_before();

@@ -328,6 +328,8 @@ PACKED = [
     ([1, 1, 1, 1], [1, 129, 1000, 16], 4, 1, 128, True),
     ([3] * 70, None, 2, 1, 64, True),               # more sequences than a warp has lanes
     ([40, 700] * 40, None, 2, 2, 128, True),
+    ([300] + [260] * 40, [300] + [0] * 40, 40, 40, 64, True),  # many items without keys behind some with
+    ([300] + [260] * 40 + [129], [300] + [0] * 40 + [129], 24, 4, 128, False),
 ]
 
 
