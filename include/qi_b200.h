@@ -316,11 +316,17 @@ int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk
  * with V.  lse (optional, fp32 [total_q, heads]): log of the sum of
  * exp(scale q.k), -inf where no key is seen.  Rows of out (and lse) outside
  * every sequence are left as they were.  Keys and values inside a sequence
- * have to be finite. */
+ * have to be finite.  With a workspace of the size that
+ * qi_b200_attention_packed_workspace_bytes names (0: none is of use), items
+ * may be cut over several SMs where they do not fill the device evenly; it
+ * needs no initialization and may be used again by the next call on the
+ * stream.  Without one (null, or smaller) nothing is cut. */
+int qi_b200_attention_packed_workspace_bytes(int n_seq, int total_q, int total_k, int heads, int kv_heads, int head_dim,
+                                             size_t* bytes);
 int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
                              void* out, long long ldo, float* lse, const int* cu_q, const int* cu_k, int n_seq,
                              int total_q, int total_k, int heads, int kv_heads, int head_dim, int causal, float scale,
-                             cudaStream_t stream);
+                             void* workspace, size_t workspace_bytes, cudaStream_t stream);
 
 /* Attention of one new token per sequence over a paged cache: row b of q
  * attends the first lengths[b] tokens (int32, device) of sequence b, whose

@@ -73,6 +73,7 @@ struct PackedParams {
   __nv_bfloat16* out;
   long long ldo;
   float* lse;        // [total_q, heads] or nullptr
+  float* ws;         // partial results and records, or nullptr: items are never cut
 };
 
 // Shared-memory descriptors as two words.  The high word is a constant (8-row
@@ -142,13 +143,16 @@ struct PackedCfg {
   static constexpr uint32_t IDESC_O = make_idesc(kDF32, kFmtBF16, kFmtBF16, 128, D) | (1u << 16);  // B is MN-major
 };
 
-// One work item, as the scheduling warp puts it into shared memory.
+// One work item, or the part of one that falls to a CTA, as the scheduling
+// warp puts it into shared memory.
 struct PackedItem {
-  int q0, lq, k0, lk;  // first rows and lengths of the sequence
+  int q0, lq;          // first query row and length of the sequence
+  int k0, lk;          // first key row of the part; keys of the sequence from there on
   int m[2], head[2];   // first token (inside the sequence) and head of the two tiles
   int n[2];            // 128-key steps of the two tiles (0: nothing visible, or no rows)
+  int diag;            // last visible key of token i is i + diag (counted from k0), at most lk - 1
+  int part;            // -1: whole; else the CTA's workspace place that takes the partial result
   int last;            // 1: there is no item, the CTA is done
-  int pad;
 };
 constexpr int kPackedItems = 4;  // items in flight
 
@@ -158,24 +162,200 @@ __device__ __forceinline__ void packed_span(const int* cu, int b, int total, int
   len = min(max(cu[b + 1], first), total) - first;
 }
 
-// The items of this CTA, longest first, one after another into `out` (the whole warp calls it).
-template <class Put>
+// The 128-key steps of the two tiles of an item (query block `level` of sequence b).
+struct PackedGeometry {
+  int q0, lq, k0, lk, n[2];
+};
+__device__ __forceinline__ PackedGeometry packed_geometry(const PackedParams& p, int b, int level) {
+  PackedGeometry g;
+  packed_span(p.cu_q, b, p.total_q, g.q0, g.lq);
+  packed_span(p.cu_k, b, p.total_k, g.k0, g.lk);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int m = p.pair_heads ? level * 128 : level * 256 + 128 * t;
+    const int rows = min(128, g.lq - m);
+    const int visible = p.causal ? min(g.lk, m + rows + g.lk - g.lq) : g.lk;
+    g.n[t] = rows > 0 && visible > 0 ? (visible + 127) / 128 : 0;
+  }
+  return g;
+}
+
+// Steps [lo, hi) of an item (counted from its first key); whole where that is all of it.
+__device__ __forceinline__ PackedItem packed_item(const PackedParams& p, const PackedGeometry& g, int level, int hi_,
+                                                  int lo, int hi, int part) {
+  PackedItem it;
+  it.q0 = g.q0, it.lq = g.lq;
+  it.k0 = g.k0 + lo * 128, it.lk = g.lk - lo * 128;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    it.head[t] = p.pair_heads ? 2 * hi_ + t : hi_;
+    it.m[t] = p.pair_heads ? level * 128 : level * 256 + 128 * t;
+    it.n[t] = max(0, min(g.n[t], hi) - lo);
+  }
+  it.diag = p.causal ? it.lk - it.lq : 0x3fffffff - g.lq;
+  it.part = part;
+  it.last = 0;
+  return it;
+}
+
+// One partial result in the workspace: per tile 128 maxima, 128 sums and D
+// columns of 128 fp32 output elements.
+template <int D>
+__host__ __device__ constexpr int packed_part_floats() { return 2 * 128 * (D + 2); }
+// Which item a partial result belongs to; two places per CTA: 0 for an item
+// that an earlier CTA begins, 1 for one that the CTA begins and a later one goes on with.
+struct PackedRecord {
+  int used, ends;           // there is a partial result; it is the item's last
+  int row[2], rows[2], head[2];
+};
+
+// An even split pays where the longest-first order leaves SMs idle for longer
+// than writing and joining the partial results takes (about 12 us, 7 steps).
+// What that order leaves idle: at most one item per CTA, the longest; equal
+// items, what the last round lacks; falling lengths, about half the length of
+// the last round's items.
+__device__ __forceinline__ bool packed_even_split(long long steps, long long items, int longest, int G, int causal) {
+  const long long even = steps / G;
+  long long order;
+  if (items <= G) order = longest;
+  else if (!causal) order = (items + G - 1) / G * longest;
+  else order = even + static_cast<long long>(longest) * G / (2 * items);
+  return order - even > 7;
+}
+
+// The items of this CTA one after another to `put` (the whole warp calls it).
+template <int D, class Put>
 __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) {
   const int lane = threadIdx.x & 31;
   const int rows_per_item = p.pair_heads ? 128 : 256;
   const int heads_items = p.pair_heads ? p.heads / 2 : p.heads;
+  const int G = gridDim.x, me = blockIdx.x;
   auto blocks = [&](int b) {
     if (b >= p.n_seq) return 0;
     int first, len;
     packed_span(p.cu_q, b, p.total_q, first, len);
     return (len + rows_per_item - 1) / rows_per_item;
   };
+  auto steps_of = [&](int b, int level) {
+    const PackedGeometry g = packed_geometry(p, b, level);
+    return max(g.n[0], g.n[1]);
+  };
+  if (p.ws != nullptr) {
+    PackedRecord* rec = reinterpret_cast<PackedRecord*>(p.ws + 2ll * G * packed_part_floats<D>()) + 2 * me;
+    if (lane < 2) rec[lane].used = 0;
+    __syncwarp();
+    long long total = 0;
+    int longest = 0, count = 0;
+    auto seq_steps = [&](int b) {  // steps of one head item of sequence b
+      const int nb = blocks(b);
+      int sum = 0;
+      for (int level = 0; level < nb; ++level) {
+        const int s = steps_of(b, level);
+        sum += s;
+        longest = max(longest, s);
+      }
+      count += nb;
+      return sum;
+    };
+    for (int b = lane; b < p.n_seq; b += 32) total += seq_steps(b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+      count += __shfl_xor_sync(0xffffffffu, count, o);
+    }
+    total *= heads_items;
+    if (packed_even_split(total, static_cast<long long>(count) * heads_items, longest, G, p.causal)) {
+      // the steps of all items end to end (sequences in order, blocks in order,
+      // heads), cut into equal ranges of three steps or more, so that the parts of
+      // an item are those of consecutive CTAs; an item's last steps come first in it
+      const long long cuts = max(1ll, min(static_cast<long long>(G), total / 3));
+      const long long lo = total * min(static_cast<long long>(me), cuts) / cuts;
+      const long long hi = total * min(me + 1ll, cuts) / cuts;
+      auto scan = [&](long long v) {  // inclusive, over the lanes
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long u = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += u;
+        }
+        return v;
+      };
+      long long before = 0;  // steps of the sequences in front of the chunk
+      int idle = 0;          // blocks without steps so far (zeros to write: the CTAs take turns at them)
+      for (int chunk = 0; chunk < p.n_seq; chunk += 32) {
+        const long long mine = static_cast<long long>(seq_steps(chunk + lane)) * heads_items;
+        const long long end = before + scan(mine);
+        unsigned todo = __ballot_sync(0xffffffffu, end > lo && end - mine < hi && mine > 0);
+        while (todo) {
+          const int i = __ffs(todo) - 1;
+          todo &= todo - 1;
+          const int b = chunk + i, nb = blocks(b);
+          long long at = __shfl_sync(0xffffffffu, end - mine, i);
+          for (int l0 = 0; l0 < nb && at < hi; l0 += 32) {
+            const int s_lane = l0 + lane < nb ? steps_of(b, l0 + lane) : 0;
+            const long long l_end = at + scan(static_cast<long long>(s_lane) * heads_items);
+            unsigned levels = __ballot_sync(0xffffffffu, s_lane > 0 && l_end > lo &&
+                                                             l_end - static_cast<long long>(s_lane) * heads_items < hi);
+            while (levels) {
+              const int j = __ffs(levels) - 1;
+              levels &= levels - 1;
+              const int level = l0 + j;
+              const PackedGeometry g = packed_geometry(p, b, level);
+              const int s = max(g.n[0], g.n[1]);
+              const long long first = __shfl_sync(0xffffffffu, l_end, j) - static_cast<long long>(s) * heads_items;
+              int h = first < lo ? static_cast<int>((lo - first) / s) : 0;
+              for (long long u = first + static_cast<long long>(h) * s; h < heads_items && u < hi; ++h, u += s) {
+                const int from = static_cast<int>(max(0ll, lo - u));
+                const int to = static_cast<int>(min(static_cast<long long>(s), hi - u));
+                const int part = from == 0 && to == s ? -1 : (from == 0 ? 1 : 0);
+                const PackedItem it = packed_item(p, g, level, h, s - to, s - from, part);
+                if (part >= 0 && lane == 0) {
+                  PackedRecord r;
+                  r.used = 1;
+                  r.ends = to == s;
+#pragma unroll
+                  for (int t = 0; t < 2; ++t) {
+                    r.row[t] = it.q0 + it.m[t];
+                    r.rows[t] = max(0, min(128, it.lq - it.m[t]));
+                    r.head[t] = it.head[t];
+                  }
+                  rec[part] = r;
+                }
+                if (!put(it)) return;
+              }
+            }
+            at = __shfl_sync(0xffffffffu, l_end, 31);
+          }
+        }
+        before = __shfl_sync(0xffffffffu, end, 31);
+        int none = 0;
+        for (int level = 0; level < blocks(chunk + lane); ++level) none += steps_of(chunk + lane, level) == 0;
+        unsigned with = __ballot_sync(0xffffffffu, none > 0);
+        while (with) {
+          const int i = __ffs(with) - 1;
+          with &= with - 1;
+          const int b = chunk + i, nb = blocks(b);
+          for (int level = 0; level < nb; ++level) {
+            const PackedGeometry g = packed_geometry(p, b, level);
+            if (g.n[0] > 0 || g.n[1] > 0) continue;
+            for (int h = (me + idle) % G; h < heads_items; h += G)
+              if (!put(packed_item(p, g, level, h, 0, 0, -1))) return;
+            ++idle;
+          }
+        }
+      }
+      PackedItem end = {};
+      end.last = 1;
+      put(end);
+      return;
+    }
+  }
+  // longest first: level by level from the last
   int most = 0;
   for (int b = lane; b < p.n_seq; b += 32) most = max(most, blocks(b));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
   const int blocks0 = blocks(lane);
-  const int G = gridDim.x, me = blockIdx.x;
   int base = 0, round = 0;  // items before this (level, chunk); rounds of G items begun
   for (int level = most - 1; level >= 0; --level) {
     for (int chunk = 0; chunk < p.n_seq; chunk += 32) {
@@ -188,20 +368,8 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
         const int nth = idx / heads_items, hi = idx - nth * heads_items;
         unsigned mm = active;
         for (int i = 0; i < nth; ++i) mm &= mm - 1;
-        const int b = chunk + __ffs(mm) - 1;
-        PackedItem it;
-        packed_span(p.cu_q, b, p.total_q, it.q0, it.lq);
-        packed_span(p.cu_k, b, p.total_k, it.k0, it.lk);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          it.head[t] = p.pair_heads ? 2 * hi + t : hi;
-          it.m[t] = level * rows_per_item + (p.pair_heads ? 0 : 128 * t);
-          const int rows = min(128, it.lq - it.m[t]);
-          const int visible = p.causal ? min(it.lk, it.m[t] + rows + it.lk - it.lq) : it.lk;
-          it.n[t] = rows > 0 && visible > 0 ? (visible + 127) / 128 : 0;
-        }
-        it.last = it.pad = 0;
-        if (!put(it)) return;
+        const PackedGeometry g = packed_geometry(p, chunk + __ffs(mm) - 1, level);
+        if (!put(packed_item(p, g, level, hi, 0, max(g.n[0], g.n[1]), -1))) return;
       }
       base += n;
     }
@@ -288,7 +456,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 10) {
       // ---- items ----
-      packed_schedule(p, [&](const PackedItem& it) {
+      packed_schedule<D>(p, [&](const PackedItem& it) {
         const int i = n_it % kPackedItems;
         if (!mbar_wait_hot(&it_empty[i], ((n_it / kPackedItems) & 1u) ^ 1u, abort_flag, kTagPacked, 12)) return false;
         if (lane == 0) {
@@ -481,12 +649,8 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     bool ok = true;
     while (const PackedItem* it = next_item()) {
       const int steps = it->n[t];
-      int limit, first_limit;  // last visible key of this row and of the tile's first row
-      {
-        const int lk = it->lk, m = it->m[t], reach = p.causal ? m + lk - it->lq : lk - 1;
-        first_limit = min(lk - 1, reach);
-        limit = min(lk - 1, p.causal ? reach + row : reach);
-      }
+      // last visible key of this row and of the tile's first row
+      const int first_limit = min(it->lk - 1, it->m[t] + it->diag), limit = min(it->lk - 1, it->m[t] + row + it->diag);
       float m_use = -INFINITY;
       float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       for (int j = steps - 1; j >= 0; --j) {
@@ -562,6 +726,28 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       const long long first = it->q0 + it->m[t] + (warp & 3) * 32;
       __nv_bfloat16* dst = p.out + first * p.ldo + head * D;
       float* lse = p.lse != nullptr && lane < rows ? p.lse + (first + lane) * p.heads + head : nullptr;
+      if (it->part >= 0) {
+        // a part: maxima, sums and unnormalized output to the workspace, row fastest
+        float* part = p.ws + (2ll * blockIdx.x + it->part) * packed_part_floats<D>() + t * (128 * (D + 2)) + row;
+        part[0] = m_use;
+        part[128] = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+        if (steps > 0) {
+          ok = mbar_wait_hot(&o_done[t], n_items++ & 1u, abort_flag, kTagPacked, 44);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(t_o + 32 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) part[(2 + 32 * c + i) * 128] = __uint_as_float(o[i]);
+          }
+          tc_fence_before();
+        }
+        release_item();
+        continue;
+      }
       float inv = 0.f;  // a row that saw no key gives zeros
       if (steps > 0) {
         ok = mbar_wait_hot(&o_done[t], n_items++ & 1u, abort_flag, kTagPacked, 43);
@@ -617,6 +803,57 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     __syncwarp();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
+}
+
+// Joins the partial results of the items that k_attn_packed cut.  CTA (c, y)
+// looks at the item that CTA c of that kernel began and did not finish, tile
+// y / 4, 32 rows: the parts are its place 1, then place 0 of the CTAs behind it
+// up to the one that ends the item, added up in that order.  A warp per D / 8
+// columns, a lane per row.
+template <int D>
+__global__ void __launch_bounds__(256) k_attn_packed_join(const PackedParams p, int ctas) {
+  griddep_wait();
+  griddep_launch_dependents();
+  constexpr int N = D / 8;
+  const PackedRecord* rec = reinterpret_cast<const PackedRecord*>(p.ws + 2ll * ctas * packed_part_floats<D>());
+  const int c0 = blockIdx.x, t = blockIdx.y >> 2;
+  const PackedRecord r = rec[2 * c0 + 1];
+  if (!r.used) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = (blockIdx.y & 3) * 32 + lane;
+  const bool live = row < (t ? r.rows[1] : r.rows[0]);
+  if (!__any_sync(0xffffffffu, live)) return;
+  auto part = [&](int c) {
+    return p.ws + (2ll * c + (c == c0 ? 1 : 0)) * packed_part_floats<D>() + t * (128 * (D + 2)) + row;
+  };
+  int c1 = c0 + 1;
+  while (c1 < ctas - 1 && !rec[2 * c1].ends) ++c1;
+  float m = -INFINITY;
+  for (int c = c0; c <= c1; ++c) m = fmaxf(m, part(c)[0]);
+  float sum = 0.f, acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  for (int c = c0; c <= c1; ++c) {
+    const float* w = part(c);
+    if (w[0] == -INFINITY) continue;  // saw no key: nothing was written behind the sum
+    const float f = ex2_approx(w[0] - m);
+    sum = fmaf(w[128], f, sum);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = fmaf(w[(2 + warp * N + i) * 128], f, acc[i]);
+  }
+  if (!live) return;
+  const float inv = m > -INFINITY ? 1.f / sum : 0.f;
+  const long long grow = (t ? r.row[1] : r.row[0]) + row;
+  const int head = t ? r.head[1] : r.head[0];
+  __nv_bfloat16* dst = p.out + grow * p.ldo + head * D + warp * N;
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = acc[8 * i + e] * inv;
+    reinterpret_cast<uint4*>(dst)[i] = pack8(f);
+  }
+  if (p.lse != nullptr && warp == 0)
+    p.lse[grow * p.heads + head] = m > -INFINITY ? (m + log2f(sum)) * 0.69314718055994531f : -INFINITY;
 }
 
 }  // namespace qib

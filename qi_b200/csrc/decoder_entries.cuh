@@ -71,6 +71,23 @@ static int launch_rope(const RopeAxesParams& p, int cache, cudaStream_t stream) 
   return launched(launch_pdl(k_rope_axes<IL, 2>, grid, block, 0, stream, 1, p));
 }
 
+// Work items of a packed batch, at most: the partial query blocks of the
+// sequences are bounded by their number.
+static long long packed_items(int n_seq, int total_q, int heads, int kv_heads) {
+  const bool pair = heads / kv_heads % 2 == 0;
+  return (static_cast<long long>(total_q) / (pair ? 128 : 256) + n_seq) * (pair ? heads / 2 : heads);
+}
+
+// Whether a packed batch may profit from cut items (the kernel decides, it
+// knows the lengths): with more than 16 items per SM the longest-first order
+// is even enough by itself, and below 8 key steps an item is too short.
+static size_t packed_workspace(int n_seq, int total_q, int total_k, int heads, int kv_heads, int head_dim, int num_sms) {
+  if (packed_items(n_seq, total_q, heads, kv_heads) > 16ll * num_sms || total_k <= 7 * 128) return 0;
+  return static_cast<size_t>(num_sms) * 2 *
+         ((head_dim == 128 ? packed_part_floats<128>() : packed_part_floats<64>()) * sizeof(float) +
+          sizeof(PackedRecord));
+}
+
 template <int D>
 static int launch_packed(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
                          const PackedParams& p, int num_sms, cudaStream_t stream) {
@@ -89,13 +106,13 @@ static int launch_packed(const void* q, long long ldq, const void* k, long long 
                          64, 128)))
     return rc;
   if ((rc = allow_smem<&k_attn_packed<D>>(C::SMEM))) return rc;
-  // at most one item per query block and head item; partial blocks of the
-  // sequences are bounded by their number
-  const long long rows = p.pair_heads ? 128 : 256;
-  const long long items = (p.total_q / rows + p.n_seq) * (p.pair_heads ? p.heads / 2 : p.heads);
+  const long long items = packed_items(p.n_seq, p.total_q, p.heads, p.kv_heads);
   if (items > 0x7fff0000ll) return QI_B200_ETOOBIG;  // the kernel counts items in 32 bits
-  const int grid = static_cast<int>(std::min<long long>(num_sms, std::max(1ll, items)));
-  return launched(launch_pdl(k_attn_packed<D>, dim3(grid), dim3(C::THREADS), C::SMEM, stream, 1, tq, tk, tv, p));
+  // with a workspace every SM has a place in it
+  const int grid = p.ws != nullptr ? num_sms : static_cast<int>(std::min<long long>(num_sms, std::max(1ll, items)));
+  rc = launched(launch_pdl(k_attn_packed<D>, dim3(grid), dim3(C::THREADS), C::SMEM, stream, 1, tq, tk, tv, p));
+  if (rc || p.ws == nullptr) return rc;
+  return launched(launch_pdl(k_attn_packed_join<D>, dim3(grid, 8), dim3(256), 0, stream, 1, p, grid));
 }
 
 template <int D, bool FP8>
@@ -228,7 +245,7 @@ int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk
 int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
                              void* out, long long ldo, float* lse, const int* cu_q, const int* cu_k, int n_seq,
                              int total_q, int total_k, int heads, int kv_heads, int head_dim, int causal, float scale,
-                             cudaStream_t stream) {
+                             void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   if (head_dim != 64 && head_dim != 128) return QI_B200_ESHAPE;
   if (n_seq < 0 || total_q < 0 || total_k < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return QI_B200_ESHAPE;
   if (n_seq == 0 || total_q == 0) return QI_B200_OK;
@@ -239,9 +256,12 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
   if (ldq < wq || ldo < wq || ldq % 8 || ldo % 8) return QI_B200_ESHAPE;
   if (total_k > 0 && (ldk < wk || ldv < wk || ldk % 8 || ldv % 8)) return QI_B200_ESHAPE;
   if (!aligned16(q) || !aligned16(out) || (total_k > 0 && (!aligned16(k) || !aligned16(v)))) return QI_B200_EALIGN;
+  if (workspace != nullptr && !aligned16(workspace)) return QI_B200_EALIGN;
   DeviceInfo* di = nullptr;
   if (int rc = device_info(&di)) return rc;
+  const size_t need = packed_workspace(n_seq, total_q, total_k, heads, kv_heads, head_dim, di->num_sms);
   PackedParams p = {};
+  p.ws = need > 0 && workspace != nullptr && workspace_bytes >= need ? static_cast<float*>(workspace) : nullptr;
   p.cu_q = cu_q;
   p.cu_k = cu_k;
   p.n_seq = n_seq;
@@ -258,6 +278,18 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
   p.lse = lse;
   return head_dim == 128 ? launch_packed<128>(q, ldq, k, ldk, v, ldv, p, di->num_sms, stream)
                          : launch_packed<64>(q, ldq, k, ldk, v, ldv, p, di->num_sms, stream);
+}
+
+int qi_b200_attention_packed_workspace_bytes(int n_seq, int total_q, int total_k, int heads, int kv_heads, int head_dim,
+                                             size_t* bytes) {
+  if (bytes == nullptr) return QI_B200_EINVAL;
+  if ((head_dim != 64 && head_dim != 128) || n_seq < 0 || total_q < 0 || total_k < 0 || heads <= 0 || kv_heads <= 0 ||
+      heads % kv_heads)
+    return QI_B200_ESHAPE;
+  DeviceInfo* di = nullptr;
+  if (int rc = device_info(&di)) return rc;
+  *bytes = packed_workspace(n_seq, total_q, total_k, heads, kv_heads, head_dim, di->num_sms);
+  return QI_B200_OK;
 }
 
 int qi_b200_attention_paged_workspace_bytes(int head_dim, size_t* bytes) {

@@ -269,10 +269,18 @@ inline at::Tensor attention_packed(const at::Tensor& q, const at::Tensor& k, con
   same.on(out, "out"), same.on(lse, "lse");
   const c10::cuda::CUDAGuard guard(same.dev);
   at::Tensor o = given(out) ? *out : at::empty({Tq, heads * D}, q.options());
+  const int n_seq = small(cu_q.numel() - 1, "sequences");
+  size_t ws_bytes = 0;
+  done(qi_b200_attention_packed_workspace_bytes(n_seq, small(Tq, "Tq"), small(Tk, "Tk"), small(heads, "heads"),
+                                                small(kv_heads, "kv_heads"), static_cast<int>(D), &ws_bytes),
+       "qi_b200_attention_packed_workspace_bytes");
+  at::Tensor ws;
+  if (ws_bytes) ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
   done(qi_b200_attention_packed(ptr(q), ldq, ptr(k), ldk, ptr(v), ldv, ptr(o), ldo, static_cast<float*>(ptr(lse)),
-                                cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), small(cu_q.numel() - 1, "sequences"),
-                                small(Tq, "Tq"), small(Tk, "Tk"), small(heads, "heads"), small(kv_heads, "kv_heads"),
-                                static_cast<int>(D), causal, f, at::cuda::getCurrentCUDAStream(same.dev.index())),
+                                cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), n_seq, static_cast<int>(Tq),
+                                static_cast<int>(Tk), static_cast<int>(heads), static_cast<int>(kv_heads),
+                                static_cast<int>(D), causal, f, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
+                                at::cuda::getCurrentCUDAStream(same.dev.index())),
        "qi_b200_attention_packed");
   return o;
 }

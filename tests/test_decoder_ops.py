@@ -179,13 +179,18 @@ def test_c_abi_refuses_before_it_touches_the_device():
     assert rope() == _lib.EALIGN
     c.slot_stride[1] = 128
 
-    packed_ = lambda q=p, k=p, ldq=256, n=1, tq=4, heads=2, kv=1, D=128, scale=1.0, cu=p: \
-        lib.qi_b200_attention_packed(q, ldq, k, 128, p, 128, p, 256, None, cu, p, n, tq, 4, heads, kv, D, 1, scale, None)
+    packed_ = lambda q=p, k=p, ldq=256, n=1, tq=4, heads=2, kv=1, D=128, scale=1.0, cu=p, ws=None: \
+        lib.qi_b200_attention_packed(q, ldq, k, 128, p, 128, p, 256, None, cu, p, n, tq, 4, heads, kv, D, 1, scale,
+                                     ws, 1 << 30, None)
     assert packed_(n=0) == packed_(tq=0) == _lib.OK
     assert packed_(D=96) == packed_(heads=3, kv=2) == packed_(ldq=128) == packed_(ldq=260) == _lib.ESHAPE
     assert packed_(q=None) == packed_(k=None) == packed_(cu=None) == packed_(scale=0.0) == _lib.EINVAL
     assert packed_(scale=float("nan")) == _lib.EINVAL
-    assert packed_(k=p + 8) == _lib.EALIGN
+    assert packed_(k=p + 8) == packed_(ws=p + 8) == _lib.EALIGN
+    size = ref(ctypes.c_size_t())
+    assert lib.qi_b200_attention_packed_workspace_bytes(1, 4, 4, 3, 2, 128, size) == _lib.ESHAPE
+    assert lib.qi_b200_attention_packed_workspace_bytes(1, 4, 4, 2, 2, 96, size) == _lib.ESHAPE
+    assert lib.qi_b200_attention_packed_workspace_bytes(1, 4, 4, 2, 2, 128, None) == _lib.EINVAL
     assert packed_() == _lib.ECUDA
 
     paged_ = lambda q=p, B=2, heads=2, kv=1, D=128, mp=4, ld=4, ws=p, scale=1.0, nb=1 << 30: \

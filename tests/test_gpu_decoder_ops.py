@@ -328,6 +328,10 @@ PACKED = [
     ([1, 1, 1, 1], [1, 129, 1000, 16], 4, 1, 128, True),
     ([3] * 70, None, 2, 1, 64, True),               # more sequences than a warp has lanes
     ([40, 700] * 40, None, 2, 2, 128, True),
+    ([129], [9000], 2, 2, 128, True),               # few items over many keys: cut over the SMs and joined
+    ([700, 3, 0, 200], [20000, 1500, 700, 0], 6, 2, 64, True),
+    ([260, 40], [3000, 2500], 3, 1, 128, False),
+    ([2200, 300], [2200, 100], 16, 16, 128, True),  # cut, with query blocks that see no key
     ([300] + [260] * 40, [300] + [0] * 40, 40, 40, 64, True),  # many items without keys behind some with
     ([300] + [260] * 40 + [129], [300] + [0] * 40 + [129], 24, 4, 128, False),
 ]
