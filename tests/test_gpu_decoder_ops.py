@@ -159,6 +159,7 @@ def rotate_ref(x, heads, D, positions, freqs, axes, interleaved):
     (13, 3, 3, 80, (8, 8, 8), True, False, torch.int32),    # 48 of 80 elements
     (9, 2, 1, 512, (256,), True, True, torch.int32),
     (6, 1, 2, 16, (8,), True, False, torch.int32),
+    (2600, 1, 1, 16, (8,), True, True, torch.int64),
 ])
 def test_rope_axes(M, hq, hk, D, sections, shared, interleaved, idx):
     g = gen(M + D)
