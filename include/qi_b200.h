@@ -336,7 +336,7 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
  * the device status word is set (code 2).  The workspace holds partial
  * results of sequences that several SMs share; it needs no initialization and
  * may be used again by the next call on the stream. */
-int qi_b200_attention_paged_workspace_bytes(int head_dim, size_t* bytes);
+int qi_b200_attention_paged_workspace_bytes(int kv_heads, int head_dim, size_t* bytes);
 int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_cache* cache, const int* page_table,
                             long long ld_table, int max_pages, const int* lengths, void* out, long long ldo,
                             float* lse, int B, int heads, int kv_heads, int head_dim, float scale, void* workspace,

@@ -88,7 +88,7 @@ SIGNATURES = {
     "qi_b200_attention_packed": [_P, _LL, _P, _LL, _P, _LL, _P, _LL, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P,
                                  ctypes.c_size_t, _P],
     "qi_b200_attention_packed_workspace_bytes": [_I, _I, _I, _I, _I, _I, _P],
-    "qi_b200_attention_paged_workspace_bytes": [_I, _P],
+    "qi_b200_attention_paged_workspace_bytes": [_I, _I, _P],
     "qi_b200_attention_paged": [_P, _LL, _P, _P, _LL, _I, _P, _P, _LL, _P, _I, _I, _I, _I, _F, _P, ctypes.c_size_t,
                                 _P],
     "qi_b200_nvfp4_linear": [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],

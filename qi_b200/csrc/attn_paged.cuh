@@ -4,24 +4,38 @@
 // names.  Bound: HBM, every cached row is read once and serves all query
 // heads of its key head.
 //
-// Split: the work of all (sequence, key head, chunk of 16 query heads) items,
-// counted in units of kPagedUnit tokens, is laid end to end and cut into
-// gridDim.x equal ranges, one per CTA, so every SM streams the same number of
-// bytes whatever the lengths are.  An item inside one range is finished there;
-// an item cut by range borders leaves partial results (row maximum, sum,
-// unnormalized output, all fp32) in the workspace, which k_attn_paged_join
-// adds up in range order: the result does not depend on timing.
+// An item is a sequence, a group of 1 to 8 key heads and a chunk of 16 query
+// heads of each.  Where the heads of a cached token lie next to each other, the
+// warps of a CTA form one team per key head and read the same tokens together:
+// a head row of 64 to 256 bytes by itself leaves DRAM pages open for too little
+// (64 sequences of up to 8192 tokens, 8 key heads: bf16 rows of 256 bytes
+// 176 us with one head at a time, 168 / 162 / 161 with 2 / 4 / 8; E4M3 rows of
+// 128 bytes 151, 126, 121, 115).
+//
+// Split: the work of all items, counted in units of at least 16 tokens, is laid
+// end to end and cut into gridDim.x equal ranges, one per CTA, so every SM
+// streams the same number of bytes whatever the lengths are.  An item inside
+// one range is finished there; an item cut by range borders leaves partial
+// results (row maximum, sum, unnormalized output, all fp32) in the workspace,
+// which k_attn_paged_join adds up in range order: the result does not depend on
+// timing.
 //
 // Inside a CTA the warps take blocks of the range in turn.  Each warp runs
 // its own ring of cp.async stages (no barrier between warps while it streams)
-// and its own running softmax: S = Q K^T and O += P V with mma.sync m16n8k16,
-// the query heads of the item as the 16 rows.  The tensor work is a few
-// per cent of what the SM can do, so the legacy instruction is enough; what
-// counts are the bytes in flight (8 warps x 2 stages x 8 KB per SM).
+// and its own running softmax, transposed so that the query heads of a key head
+// are the 8 columns of mma.sync m16n8k16: S^T = K Q^T (16 tokens x 8 heads) and
+// O^T += V^T P^T (16 columns x 8 heads); 9 to 16 heads take two column tiles
+// over the same K and V fragments.  P^T goes from S^T's accumulator layout to
+// the operand layout with one 8 x 8 transpose per 8 tokens.  The maximum in use
+// follows only when a row outgrew it by more than 2^8, so most blocks need one
+// vote and no reduction.  The tensor work is a few per cent of what the SM can
+// do, so the legacy instruction is enough; what counts are the bytes in flight
+// (128 KB per SM) and the instructions per byte.
 //
 // E4M3 caches: codes are widened exactly to fp16 and multiplied in fp16 with
-// fp32 sums; q is scaled by a power of two per row so that it fits fp16, the
+// fp32 sums; q is scaled by a power of two per head so that it fits fp16, the
 // key scale goes into the softmax scale and the value scale into the output.
+// P is at most 2^8, inside fp16's range.
 //
 // A page index outside the cache, or a length behind the page table, reads
 // nothing: those keys take no part, and the device status word is set.
@@ -40,10 +54,9 @@
 namespace qib {
 
 constexpr unsigned int kTagPaged = 0x800u;
-constexpr int kPagedUnit = 64;      // tokens per unit of work
-constexpr int kPagedWarps = 8;
+constexpr int kPagedUnit = 64;      // tokens per unit of work, times key heads per item
 constexpr int kPagedRows = 16;      // query heads per item
-constexpr int kPagedStageBytes = 8192;
+constexpr int kPagedWarps = 8;
 
 struct PagedParams {
   const __nv_bfloat16* q;
@@ -60,11 +73,13 @@ struct PagedParams {
   const float* scale[2];                   // E4M3: k_scale, v_scale, [1] or [kv_heads]
   int scale_per_head[2];
   int B, heads, kv_heads, group, chunks;   // chunks of kPagedRows query heads per key head
+  int team_shift, groups;                  // log2 of the key heads per item; kv_heads in such groups
   int page_size, max_pages, num_pages;
+  int page_shift;                          // log2 of page_size, or -1
   float scale_log2e;
 };
 
-// Floats of one partial result: maxima, sums, output rows.
+// Floats of one partial result of one key head: maxima, sums, output rows.
 template <int D>
 __host__ __device__ constexpr int paged_part_floats() { return kPagedRows * (D + 2); }
 
@@ -77,7 +92,11 @@ __device__ __forceinline__ int paged_length(const PagedParams& p, int b) {
   }
   return n < 0 ? 0 : n;
 }
-__device__ __forceinline__ int paged_units(int len) { return (len + kPagedUnit - 1) / kPagedUnit; }
+__device__ __forceinline__ int paged_unit(const PagedParams& p) { return max(16, kPagedUnit >> p.team_shift); }
+__device__ __forceinline__ int paged_units(const PagedParams& p, int len) {
+  const int n = paged_unit(p);
+  return (len + n - 1) / n;
+}
 
 // Ranges that T units are cut into: none of them is empty, so the partial
 // results of an item are those of consecutive CTAs.
@@ -116,6 +135,12 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Transpose of an 8 x 8 matrix of 16-bit elements, a row of it in every 4 lanes.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 // Two E4M3 codes (low 16 bits) -> two fp16, exact.
 __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t v) {
   uint32_t r;
@@ -137,13 +162,13 @@ template <int D, bool FP8>
 struct PagedCfg {
   static constexpr int ELT = FP8 ? 1 : 2;
   static constexpr int ROW = D * ELT;                       // bytes of one cached head row
-  static constexpr int BT = kPagedStageBytes / (2 * ROW);   // tokens per block: 16 ... 64
+  static constexpr int WARPS = kPagedWarps;
+  static constexpr int STAGE = ROW == 64 ? 4096 : 8192;
+  static constexpr int BT = STAGE / (2 * ROW);              // tokens per block: 16 or 32
   static constexpr int CH = ROW / 16;                       // 16-byte chunks per row: 4, 8 or 16
-  static constexpr int STAGES = 3;
-  static constexpr int THREADS = kPagedWarps * 32;
-  static constexpr int RING = kPagedWarps * STAGES * kPagedStageBytes;
-  static constexpr int MERGE = kPagedWarps * kPagedRows * (D + 2) * 4;
-  static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + 256;
+  static constexpr int STAGES = 24576 / STAGE;              // 192 KB in all
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int RING = WARPS * STAGES * STAGE;
   // byte offset of chunk c of row r: 128-byte lines whose 16-byte chunks are
   // permuted so that the 8 rows ldmatrix reads at once hit 8 different chunks
   __device__ static __forceinline__ uint32_t at(int r, int c) {
@@ -151,29 +176,34 @@ struct PagedCfg {
     else return r * ROW + ((c ^ ((r >> 1) & 3)) << 4);
   }
 };
+template <int D, bool FP8, int HT>
+__host__ __device__ constexpr int paged_smem() {
+  const int merge = PagedCfg<D, FP8>::WARPS * 8 * HT * (D + 2) * 4;
+  return (PagedCfg<D, FP8>::RING > merge ? PagedCfg<D, FP8>::RING : merge) + 256;
+}
 
-// ROWS8: at most 8 query heads per item (rows 8-15 of the MMA are zero).
-template <int D, bool FP8, bool ROWS8>
-__global__ void __launch_bounds__(kPagedWarps * 32, 1) k_attn_paged(const PagedParams p) {
+// HT column tiles of 8 query heads per item: 1 or 2.
+template <int D, bool FP8, int HT>
+__global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(const PagedParams p) {
   using C = PagedCfg<D, FP8>;
-  constexpr int BT = C::BT, ST = C::STAGES;
-  constexpr int NT = D / 8;        // output column tiles
-  constexpr int NR = ROWS8 ? 1 : 2;
+  constexpr int BT = C::BT, ST = C::STAGES, W = C::WARPS;
+  constexpr int KS = D / 16;       // 16-column steps of a head
+  constexpr int R = 8 * HT;        // heads of an item
   extern __shared__ __align__(128) uint8_t paged_sm[];
-  __shared__ long long scan[kPagedWarps];
+  __shared__ long long scan[W];
   __shared__ int start_b;
   __shared__ long long start_u;
-  __shared__ uint32_t masks[kPagedWarps][ST][2];
+  __shared__ uint32_t masks[W][ST];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_wait();
   griddep_launch_dependents();
 
   // the range of this CTA and the sequence it starts in
-  const long long per_unit = static_cast<long long>(p.kv_heads) * p.chunks;
+  const long long per_unit = static_cast<long long>(p.groups) * p.chunks;
   const int per_thread = (p.B + C::THREADS - 1) / C::THREADS;
   const int b_lo = min(p.B, tid * per_thread), b_hi = min(p.B, b_lo + per_thread);
   long long mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += paged_units(paged_length(p, b)) * per_unit;
+  for (int b = b_lo; b < b_hi; ++b) mine += paged_units(p, paged_length(p, b)) * per_unit;
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -184,7 +214,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_attn_paged(const PagedP
   __syncthreads();
   long long T = 0, before = 0;
 #pragma unroll
-  for (int w = 0; w < kPagedWarps; ++w) {
+  for (int w = 0; w < W; ++w) {
     if (w < warp) before += scan[w];
     T += scan[w];
   }
@@ -196,7 +226,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_attn_paged(const PagedP
   if (u < u_end && before <= u && u < before + mine) {
     long long at = before;
     for (int b = b_lo; b < b_hi; ++b) {
-      const long long n = paged_units(paged_length(p, b)) * per_unit;
+      const long long n = paged_units(p, paged_length(p, b)) * per_unit;
       if (u < at + n) {
         start_b = b;
         start_u = at;
@@ -209,136 +239,159 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_attn_paged(const PagedP
   if (u >= u_end) return;
   int b = start_b;
   long long b_first = start_u;  // first unit of sequence b
-  uint8_t* ring = paged_sm + warp * ST * kPagedStageBytes;
-  const uint32_t ring_u = smem_u32(ring);
+  const uint32_t ring_u = smem_u32(paged_sm + warp * ST * C::STAGE);
   const int g = lane >> 2, t4 = lane & 3;
+  const bool whole_pages = p.page_shift >= 0 && (1 << p.page_shift) >= BT;  // blocks start at multiples of BT
 
   while (u < u_end) {
     int len = paged_length(p, b);
-    int n_units = paged_units(len);
+    int n_units = paged_units(p, len);
     while (u >= b_first + n_units * per_unit) {  // next sequence with keys
       b_first += n_units * per_unit;
       ++b;
       len = paged_length(p, b);
-      n_units = paged_units(len);
+      n_units = paged_units(p, len);
     }
     const long long rel = u - b_first;
-    const int item = static_cast<int>(rel / n_units);           // key head and chunk
+    const int item = static_cast<int>(rel / n_units);           // group of key heads, and chunk
     const int unit0 = static_cast<int>(rel - static_cast<long long>(item) * n_units);
     const int unit1 = static_cast<int>(min(static_cast<long long>(n_units), unit0 + (u_end - u)));
-    const int kvh = item / p.chunks, chunk = item - kvh * p.chunks;
-    const int head0 = kvh * p.group + chunk * kPagedRows;
+    const int kv_group = item / p.chunks, chunk = item - kv_group * p.chunks;
     const int rows = min(kPagedRows, p.group - chunk * kPagedRows);
-    const int tok0 = unit0 * kPagedUnit, tok1 = min(len, unit1 * kPagedUnit);
+    const int tok0 = unit0 * paged_unit(p), tok1 = min(len, unit1 * paged_unit(p));
     u += unit1 - unit0;
+    // this warp's key head, and the blocks of its team: tok0 + (mate + i * mates) * BT
+    const int team = warp & ((1 << p.team_shift) - 1), mate = warp >> p.team_shift, mates = W >> p.team_shift;
+    const int kvh = (kv_group << p.team_shift) + team;
+    const int head0 = kvh * p.group + chunk * kPagedRows;
 
-    // Q as the A operand, rows g and g + 8
-    uint32_t qa[D / 16][4];
-    float row_scale[2] = {1.f, 1.f};
-    {
-      float qmax[2] = {0.f, 0.f};
-      uint32_t raw[D / 16][4];
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v = 0;
-            if (r < NR && g + 8 * r < rows) {
-              // fp16 path: the thread's 4 columns of a 16-column step are consecutive (as its 4 codes of K are)
-              const int col = ks * 16 + (FP8 ? 4 * t4 + 2 * h : 2 * t4 + 8 * h);
-              v = *reinterpret_cast<const uint32_t*>(p.q + static_cast<long long>(b) * p.ldq +
-                                                     static_cast<long long>(head0 + g + 8 * r) * D + col);
-            }
-            raw[ks][r + 2 * h] = v;
-            if (FP8) {
-              const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-              qmax[r] = fmaxf(qmax[r], fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-          }
-      if (FP8) {
-        float down[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          qmax[r] = fmaxf(qmax[r], __shfl_xor_sync(0xffffffffu, qmax[r], 1));
-          qmax[r] = fmaxf(qmax[r], __shfl_xor_sync(0xffffffffu, qmax[r], 2));
-          // 2^e with e the exponent of the row's largest element, kept so that 2^-e is a normal number
-          int e = static_cast<int>(__float_as_uint(qmax[r]) >> 23) - 127;
-          e = max(-100, min(100, e));
-          row_scale[r] = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-          down[r] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        }
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks][i]));
-            qa[ks][i] = pack_pair<true>(f.x * down[i & 1], f.y * down[i & 1]);
-          }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) qa[ks][i] = raw[ks][i];
-      }
-    }
-    float sl2[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-      sl2[r] = p.scale_log2e * (FP8 ? row_scale[r] * p.scale[0][p.scale_per_head[0] ? kvh : 0] : 1.f);
-
-    // this warp's blocks: tok0 + (warp + i * kPagedWarps) * BT
     const int n_blocks = (tok1 - tok0 + BT - 1) / BT;
-    const int my_blocks = n_blocks > warp ? (n_blocks - warp - 1) / kPagedWarps + 1 : 0;
+    const int my_blocks = n_blocks > mate ? (n_blocks - mate - 1) / mates + 1 : 0;
     const int* pg = p.pages + static_cast<long long>(b) * p.ld_pages;
+    constexpr int RPI = 32 / C::CH;       // rows copied per instruction
+    const int row0 = lane / C::CH, ch = lane % C::CH;
+    const uint8_t* lane_src[2];           // this lane's chunk of the first rows of page 0
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      lane_src[c] = p.cache[c] + kvh * p.head_stride[c] + row0 * p.slot_stride[c] + ch * 16;
     auto issue = [&](int i) {
       const int st = i % ST;
-      const int t0 = tok0 + (warp + i * kPagedWarps) * BT;
+      const int t0 = tok0 + (mate + i * mates) * BT;
+      if (whole_pages) {
+        // the block lies in one page: one look-up, rows at fixed distances
+        const int pi = t0 >> p.page_shift, place = t0 - (pi << p.page_shift);
+        const int page = pg[pi];
+        const bool good = page >= 0 && page < p.num_pages;
+        if (!good) record_error(kDevBadIndex, kTagPaged, 2);
+        const int n = good ? min(BT, tok1 - t0) : 0;
+        if (lane == 0) masks[warp][st] = n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 #pragma unroll
-      for (int half = 0; half < (BT + 31) / 32; ++half) {
-        constexpr int R = BT < 32 ? BT : 32;  // rows whose addresses the lanes look up at once
-        const int tok = t0 + half * 32 + (lane % R);
-        long long off[2] = {0, 0};
-        bool ok = tok < tok1;
-        if (ok) {
-          const int pi = tok / p.page_size, place = tok - pi * p.page_size;
-          const int page = pg[pi];
-          if (page < 0 || page >= p.num_pages) {
-            record_error(kDevBadIndex, kTagPaged, 2);
-            ok = false;
-          } else {
+        for (int c = 0; c < 2; ++c) {
+          const uint8_t* src = lane_src[c];
+          if (good) src += page * p.page_stride[c] + place * p.slot_stride[c];
+          const long long step = RPI * p.slot_stride[c];
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-              off[c] = page * p.page_stride[c] + place * p.slot_stride[c] + kvh * p.head_stride[c];
+          for (int i2 = 0; i2 < BT / RPI; ++i2) {
+            const int r = i2 * RPI + row0;
+            cp_async16(ring_u + st * C::STAGE + c * (C::STAGE / 2) + C::at(r, ch), src + i2 * step, r < n);
           }
         }
-        const uint32_t m = __ballot_sync(0xffffffffu, ok);
-        if (lane == 0) masks[warp][st][half] = BT < 32 ? (m & ((1u << (BT & 31)) - 1u)) : m;
-        constexpr int RPI = 32 / C::CH;       // rows copied per instruction
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i2 = 0; i2 < R / RPI; ++i2) {
-            const int r = i2 * RPI + lane / C::CH, ch = lane % C::CH;
-            const long long o = __shfl_sync(0xffffffffu, off[c], r);
-            cp_async16(ring_u + st * kPagedStageBytes + c * (kPagedStageBytes / 2) + C::at(half * 32 + r, ch),
-                       p.cache[c] + o + ch * 16, (m >> r) & 1u);
-          }
+        return;
       }
+      // any page size: every lane looks up a token, the copies take the addresses from there
+      const int tok = t0 + (lane % BT);
+      long long off[2] = {0, 0};
+      bool ok = tok < tok1;
+      if (ok) {
+        const int pi = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size;
+        const int place = tok - pi * p.page_size;
+        const int page = pg[pi];
+        if (page < 0 || page >= p.num_pages) {
+          record_error(kDevBadIndex, kTagPaged, 2);
+          ok = false;
+        } else {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            off[c] = page * p.page_stride[c] + place * p.slot_stride[c] + kvh * p.head_stride[c];
+        }
+      }
+      const uint32_t m = __ballot_sync(0xffffffffu, ok);
+      if (lane == 0) masks[warp][st] = m;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i2 = 0; i2 < BT / RPI; ++i2) {
+          const int r = i2 * RPI + row0;
+          const long long o = __shfl_sync(0xffffffffu, off[c], r);
+          cp_async16(ring_u + st * C::STAGE + c * (C::STAGE / 2) + C::at(r, ch), p.cache[c] + o + ch * 16,
+                     (m >> r) & 1u);
+        }
     };
-
-    float o[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
-    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i) {
       if (i < my_blocks) issue(i);
       cp_async_commit();
     }
+
+    // Q^T as the B operand: head 8 h + g, columns of a 16-column step by the lane
+    uint32_t qb[HT][KS][2];
+    float sl2[HT][2];  // scale of heads 8 h + 2 t4, 8 h + 2 t4 + 1, in powers of two
+#pragma unroll
+    for (int h = 0; h < HT; ++h) {
+      float qmax = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          // fp16 path: the lane's 4 columns are consecutive, as its 4 codes of K are
+          const int col = ks * 16 + (FP8 ? 4 * t4 + 2 * j : 2 * t4 + 8 * j);
+          uint32_t v = 0;
+          if (8 * h + g < rows)
+            v = *reinterpret_cast<const uint32_t*>(p.q + static_cast<long long>(b) * p.ldq +
+                                                   static_cast<long long>(head0 + 8 * h + g) * D + col);
+          qb[h][ks][j] = v;
+          if (FP8) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+            qmax = fmaxf(qmax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+      float up = 1.f;
+      if (FP8) {
+        qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, 1));
+        qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, 2));
+        // 2^e with e the exponent of the row's largest element, kept so that 2^-e is a normal number
+        int e = static_cast<int>(__float_as_uint(qmax) >> 23) - 127;
+        e = max(-100, min(100, e));
+        up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qb[h][ks][j]));
+            qb[h][ks][j] = pack_pair<true>(f.x * down, f.y * down);
+          }
+      }
+      const float base = p.scale_log2e * (FP8 ? p.scale[0][p.scale_per_head[0] ? kvh : 0] : 1.f);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) sl2[h][j] = base * (FP8 ? __shfl_sync(0xffffffffu, up, 4 * (2 * t4 + j)) : 1.f);
+    }
+
+    float o[HT][KS][4];
+#pragma unroll
+    for (int h = 0; h < HT; ++h)
+#pragma unroll
+      for (int n = 0; n < KS; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[h][n][i] = 0.f;
+    float mx[HT][2], sum[HT][2];
+#pragma unroll
+    for (int h = 0; h < HT; ++h)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        mx[h][j] = -INFINITY;
+        sum[h][j] = 0.f;
+      }
 #pragma unroll 1
     for (int i = 0; i < my_blocks; ++i) {
       __syncwarp();  // every lane has read stage (i - 1) % ST, which is filled next
@@ -346,174 +399,162 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_attn_paged(const PagedP
       cp_async_commit();
       cp_async_wait<ST - 1>();
       __syncwarp();
-      const uint32_t sk = ring_u + (i % ST) * kPagedStageBytes, sv = sk + kPagedStageBytes / 2;
-
-      // S = Q K^T, 8 tokens per tile
-      float s[BT / 8][4];
+      const uint32_t sk = ring_u + (i % ST) * C::STAGE, sv = sk + C::STAGE / 2;
+      const uint32_t mask = masks[warp][i % ST];
 #pragma unroll
-      for (int n = 0; n < BT / 8; ++n)
+      for (int tb = 0; tb < BT / 16; ++tb) {
+        // S^T = K Q^T of 16 tokens
+        float s[HT][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
-      if constexpr (!FP8) {
+        for (int h = 0; h < HT; ++h)
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
+          for (int j = 0; j < 4; ++j) s[h][j] = 0.f;
+        if constexpr (!FP8) {
 #pragma unroll
-          for (int n = 0; n < BT / 16; ++n) {
-            uint32_t k[4];  // (tokens 0-7, 8-15) x (dims 0-7, 8-15)
-            ldsm_x4(k, sk + C::at(n * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
-            mma_16816<false>(s[2 * n], qa[ks], k[0], k[1]);
-            mma_16816<false>(s[2 * n + 1], qa[ks], k[2], k[3]);
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t k[4];  // (tokens 0-7, 8-15) of columns 0-7, then of 8-15
+            ldsm_x4(k, sk + C::at(tb * 16 + (lane & 15), ks * 2 + (lane >> 4)));
+#pragma unroll
+            for (int h = 0; h < HT; ++h) mma_16816<false>(s[h], k, qb[h][ks][0], qb[h][ks][1]);
           }
-      } else {
+        } else {
 #pragma unroll
-        for (int kg = 0; kg < D / 32; ++kg)
+          for (int kg = 0; kg < KS / 2; ++kg) {
+            uint32_t k[4];  // (tokens 0-7, 8-15) of columns 0-15, then of 16-31; 4 codes per register
+            ldsm_x4(k, sk + C::at(tb * 16 + (lane & 15), kg * 2 + (lane >> 4)));
 #pragma unroll
-          for (int n = 0; n < BT / 16; ++n) {
-            uint32_t k[4];  // (tokens 0-7, 8-15) x (dims 0-15, 16-31), 4 codes per register
-            ldsm_x4(k, sk + C::at(n * 16 + (lane & 7) + ((lane >> 4) << 3), kg * 2 + ((lane >> 3) & 1)));
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t a[4] = {e4m3x2_to_half2(k[2 * j]), e4m3x2_to_half2(k[2 * j + 1]),
+                                     e4m3x2_to_half2(k[2 * j] >> 16), e4m3x2_to_half2(k[2 * j + 1] >> 16)};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mma_16816<true>(s[2 * n + (j >> 1)], qa[kg * 2 + (j & 1)], e4m3x2_to_half2(k[j]),
-                              e4m3x2_to_half2(k[j] >> 16));
-          }
-      }
-
-      // running softmax, in powers of two
-      float nm[2] = {mx[0], mx[1]};
-      uint32_t mk[2] = {masks[warp][i % ST][0], BT > 32 ? masks[warp][i % ST][1] : 0u};
-#pragma unroll
-      for (int n = 0; n < BT / 8; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int tok = n * 8 + 2 * t4 + j;
-          const bool ok = (mk[tok >> 5] >> (tok & 31)) & 1u;
-#pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            const float v = ok ? s[n][2 * r + j] * sl2[r] : -INFINITY;
-            s[n][2 * r + j] = v;
-            nm[r] = fmaxf(nm[r], v);
-          }
-        }
-      bool grew = false;
-#pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        nm[r] = fmaxf(nm[r], __shfl_xor_sync(0xffffffffu, nm[r], 1));
-        nm[r] = fmaxf(nm[r], __shfl_xor_sync(0xffffffffu, nm[r], 2));
-        grew |= nm[r] > mx[r];
-      }
-      if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const float f = nm[r] > mx[r] ? ex2_approx(mx[r] - nm[r]) : 1.f;  // 2^-inf = 0: nothing summed yet
-          mx[r] = nm[r];
-          sum[r] *= f;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            o[n][2 * r] *= f;
-            o[n][2 * r + 1] *= f;
-          }
-        }
-      }
-      uint32_t pa[BT / 16][4];
-#pragma unroll
-      for (int n = 0; n < BT / 8; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          uint32_t v = 0;
-          if (r < NR) {
-            const float base = mx[r] == -INFINITY ? 0.f : mx[r];
-            const float e0 = ex2_approx(s[n][2 * r] - base), e1 = ex2_approx(s[n][2 * r + 1] - base);
-            sum[r] += e0 + e1;
-            v = pack_pair<FP8>(e0, e1);
-          }
-          pa[n >> 1][(n & 1) * 2 + r] = v;
-        }
-
-      // O += P V
-      if constexpr (!FP8) {
-#pragma unroll
-        for (int ks = 0; ks < BT / 16; ++ks)
-#pragma unroll
-          for (int n = 0; n < D / 16; ++n) {
-            uint32_t v[4];  // (tokens 0-7, 8-15) x (dims 0-7, 8-15), transposed
-            ldsm_x4_t(v, sv + C::at(ks * 16 + (lane & 15), n * 2 + (lane >> 4)));
-            mma_16816<false>(o[2 * n], pa[ks], v[0], v[1]);
-            mma_16816<false>(o[2 * n + 1], pa[ks], v[2], v[3]);
-          }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < BT / 16; ++ks)
-#pragma unroll
-          for (int n = 0; n < D / 32; ++n) {
-            uint32_t v[4];  // (tokens 0-7, 8-15) x (dims 0-15, 16-31); a register: 2 tokens x 2 dims
-            ldsm_x4_t(v, sv + C::at(ks * 16 + (lane & 15), n * 2 + (lane >> 4)));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              // even dims (bytes 0, 2) and odd dims (bytes 1, 3) of the 16 make one column tile each
-              mma_16816<true>(o[4 * n + 2 * h], pa[ks], e4m3x2_to_half2(__byte_perm(v[2 * h], 0, 0x4420)),
-                              e4m3x2_to_half2(__byte_perm(v[2 * h + 1], 0, 0x4420)));
-              mma_16816<true>(o[4 * n + 2 * h + 1], pa[ks], e4m3x2_to_half2(__byte_perm(v[2 * h], 0, 0x4431)),
-                              e4m3x2_to_half2(__byte_perm(v[2 * h + 1], 0, 0x4431)));
+              for (int h = 0; h < HT; ++h) mma_16816<true>(s[h], a, qb[h][2 * kg + j][0], qb[h][2 * kg + j][1]);
             }
           }
+        }
+        // running softmax: elements (token g, g + 8) x (head 2 t4, 2 t4 + 1)
+        const bool ok0 = (mask >> (tb * 16 + g)) & 1u, ok1 = (mask >> (tb * 16 + 8 + g)) & 1u;
+        bool grew = false;
+#pragma unroll
+        for (int h = 0; h < HT; ++h)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[h][j] = ok0 ? s[h][j] * sl2[h][j] : -INFINITY;
+            s[h][2 + j] = ok1 ? s[h][2 + j] * sl2[h][j] : -INFINITY;
+            grew |= fmaxf(s[h][j], s[h][2 + j]) > mx[h][j] + 8.f;
+          }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+          for (int h = 0; h < HT; ++h)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float nm = fmaxf(mx[h][j], fmaxf(s[h][j], s[h][2 + j]));
+              nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, 4));
+              nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, 8));
+              nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, 16));
+              const float f = nm > mx[h][j] ? ex2_approx(mx[h][j] - nm) : 1.f;  // 2^-inf = 0: nothing summed yet
+              mx[h][j] = nm;
+              sum[h][j] *= f;
+#pragma unroll
+              for (int n = 0; n < KS; ++n) {
+                o[h][n][j] *= f;
+                o[h][n][2 + j] *= f;
+              }
+            }
+        }
+        uint32_t pb[HT][2];
+#pragma unroll
+        for (int h = 0; h < HT; ++h) {
+          const float m0 = mx[h][0] == -INFINITY ? 0.f : mx[h][0], m1 = mx[h][1] == -INFINITY ? 0.f : mx[h][1];
+          const float e00 = ex2_approx(s[h][0] - m0), e01 = ex2_approx(s[h][1] - m1);
+          const float e10 = ex2_approx(s[h][2] - m0), e11 = ex2_approx(s[h][3] - m1);
+          sum[h][0] += e00 + e10;
+          sum[h][1] += e01 + e11;
+          pb[h][0] = transpose8x8(pack_pair<FP8>(e00, e01));
+          pb[h][1] = transpose8x8(pack_pair<FP8>(e10, e11));
+        }
+        // O^T += V^T P^T
+        if constexpr (!FP8) {
+#pragma unroll
+          for (int n = 0; n < KS; ++n) {
+            uint32_t v[4];  // columns (0-7, 8-15) of tokens 0-7, then of 8-15, transposed
+            ldsm_x4_t(v, sv + C::at(tb * 16 + (lane & 7) + ((lane >> 4) << 3), n * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int h = 0; h < HT; ++h) mma_16816<false>(o[h][n], v, pb[h][0], pb[h][1]);
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < KS / 2; ++n) {
+            uint32_t v[4];  // tokens (0-7, 8-15) of columns 0-15, then of 16-31; a register: 2 tokens x 2 columns
+            ldsm_x4_t(v, sv + C::at(tb * 16 + (lane & 15), n * 2 + (lane >> 4)));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              // rows 0-7 of the tile are the even columns of the 16 (bytes 0, 2), rows 8-15 the odd ones (1, 3)
+              const uint32_t a[4] = {e4m3x2_to_half2(__byte_perm(v[2 * j], 0, 0x4420)),
+                                     e4m3x2_to_half2(__byte_perm(v[2 * j], 0, 0x4431)),
+                                     e4m3x2_to_half2(__byte_perm(v[2 * j + 1], 0, 0x4420)),
+                                     e4m3x2_to_half2(__byte_perm(v[2 * j + 1], 0, 0x4431))};
+#pragma unroll
+              for (int h = 0; h < HT; ++h) mma_16816<true>(o[h][2 * n + j], a, pb[h][0], pb[h][1]);
+            }
+          }
+        }
       }
     }
     cp_async_wait<0>();
     __syncthreads();  // the rings are free: they take the warps' results
 
-    // the warps' results -> shared memory: maxima, sums, rows
+    // the warps' results -> shared memory: rows, maxima, sums
     float* mg = reinterpret_cast<float*>(paged_sm);
-    float* mg_m = mg + kPagedWarps * kPagedRows * D;
-    float* mg_l = mg_m + kPagedWarps * kPagedRows;
+    float* mg_m = mg + W * R * D;
+    float* mg_l = mg_m + W * R;
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-      const int row = g + 8 * r;
-      if (t4 == 0) {
-        mg_m[warp * kPagedRows + row] = mx[r];
-        mg_l[warp * kPagedRows + row] = sum[r];
-      }
-      float* dst = mg + (warp * kPagedRows + row) * D;
+    for (int h = 0; h < HT; ++h)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if constexpr (!FP8) {
-          *reinterpret_cast<float2*>(dst + n * 8 + 2 * t4) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
-        } else {
-          const int d0 = (n >> 1) * 16 + 4 * t4 + (n & 1);  // column tiles hold the even or the odd dims of 16
-          dst[d0] = o[n][2 * r];
-          dst[d0 + 2] = o[n][2 * r + 1];
+      for (int j = 0; j < 2; ++j) {
+        float l = sum[h][j];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int row = 8 * h + 2 * t4 + j;
+        if (g == 0) {
+          mg_m[warp * R + row] = mx[h][j];
+          mg_l[warp * R + row] = l;
+        }
+        float* dst = mg + (warp * R + row) * D;
+#pragma unroll
+        for (int n = 0; n < KS; ++n) {
+          dst[n * 16 + (FP8 ? 2 * g : g)] = o[h][n][j];
+          dst[n * 16 + (FP8 ? 2 * g + 1 : g + 8)] = o[h][n][2 + j];
         }
       }
-    }
     __syncthreads();
     const bool whole = unit0 == 0 && unit1 == n_units;
-    float* part = p.ws + (2ll * blockIdx.x + (unit0 == 0 ? 1 : 0)) * paged_part_floats<D>();
-    const float v_scale = FP8 ? p.scale[1][p.scale_per_head[1] ? kvh : 0] : 1.f;
-    for (int i = tid; i < rows * (D / 2); i += C::THREADS) {
-      const int row = i / (D / 2), d = (i - row * (D / 2)) * 2;
+    float* parts = p.ws + ((2ll * blockIdx.x + (unit0 == 0 ? 1 : 0)) << p.team_shift) * paged_part_floats<D>();
+    for (int i = tid; i < (rows * (D / 2)) << p.team_shift; i += C::THREADS) {
+      const int r = i / (D / 2), d = (i - r * (D / 2)) * 2;
+      const int of = r / rows, row = r - of * rows;  // key head of the group, query head of its chunk
+      const int kv = (kv_group << p.team_shift) + of, head = kv * p.group + chunk * kPagedRows + row;
+      const float v_scale = FP8 ? p.scale[1][p.scale_per_head[1] ? kv : 0] : 1.f;
       float m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) m = fmaxf(m, mg_m[w * kPagedRows + row]);
+      for (int w = of; w < W; w += 1 << p.team_shift) m = fmaxf(m, mg_m[w * R + row]);
       const float base = m == -INFINITY ? 0.f : m;
       float l = 0.f;
       float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
-        const float f = ex2_approx(mg_m[w * kPagedRows + row] - base);
-        l = fmaf(mg_l[w * kPagedRows + row], f, l);
-        const float2 v = *reinterpret_cast<const float2*>(mg + (w * kPagedRows + row) * D + d);
+      for (int w = of; w < W; w += 1 << p.team_shift) {
+        const float f = ex2_approx(mg_m[w * R + row] - base);
+        l = fmaf(mg_l[w * R + row], f, l);
+        const float2 v = *reinterpret_cast<const float2*>(mg + (w * R + row) * D + d);
         acc.x = fmaf(v.x, f, acc.x);
         acc.y = fmaf(v.y, f, acc.y);
       }
       if (whole) {
         const float inv = l > 0.f ? v_scale / l : 0.f;
-        *reinterpret_cast<__nv_bfloat162*>(p.out + static_cast<long long>(b) * p.ldo +
-                                           static_cast<long long>(head0 + row) * D + d) =
-            __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+        *reinterpret_cast<__nv_bfloat162*>(p.out + static_cast<long long>(b) * p.ldo + static_cast<long long>(head) * D +
+                                           d) = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
         if (p.lse != nullptr && d == 0)
-          p.lse[static_cast<long long>(b) * p.heads + head0 + row] = (m + log2f(l)) * 0.69314718055994531f;
+          p.lse[static_cast<long long>(b) * p.heads + head] = (m + log2f(l)) * 0.69314718055994531f;
       } else {
+        float* part = parts + of * paged_part_floats<D>();
         if (d == 0) {
           part[row] = m;
           part[kPagedRows + row] = l;
@@ -526,20 +567,23 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_attn_paged(const PagedP
 }
 
 // Adds up the partial results of the items that were cut, and writes the rows
-// of sequences without keys (zeros).  One CTA per (sequence, query head), one
-// thread per two columns; ctas is the first kernel's grid.
+// of sequences without keys (zeros).  One CTA per (sequence, query head); its
+// warps take the parts in turn (a lane D / 32 columns, the maximum in use as
+// above) and add their sums up in warp order.  ctas is the first kernel's grid.
+constexpr int kPagedJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(D / 2 < 32 ? 32 : D / 2) k_attn_paged_join(const PagedParams p, int ctas) {
-  __shared__ long long red[2][4];
+__global__ void __launch_bounds__(kPagedJoinWarps * 32) k_attn_paged_join(const PagedParams p, int ctas) {
+  constexpr int N = D / 32;
+  __shared__ float sm_m[kPagedJoinWarps], sm_l[kPagedJoinWarps], sm_o[kPagedJoinWarps][D];
   griddep_wait();
   griddep_launch_dependents();
-  const int b = blockIdx.y, head = blockIdx.x;
+  const int b = blockIdx.y, head = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int kvh = head / p.group, in_group = head - kvh * p.group;
   const int chunk = in_group / kPagedRows, row = in_group - chunk * kPagedRows;
-  const long long per_unit = static_cast<long long>(p.kv_heads) * p.chunks;
+  const long long per_unit = static_cast<long long>(p.groups) * p.chunks;
   long long before = 0, T = 0;
-  for (int i = threadIdx.x; i < p.B; i += blockDim.x) {
-    const long long n = paged_units(paged_length(p, i)) * per_unit;
+  for (int i = lane; i < p.B; i += 32) {  // every warp for itself: no barrier
+    const long long n = paged_units(p, paged_length(p, i)) * per_unit;
     T += n;
     if (i < b) before += n;
   }
@@ -548,46 +592,57 @@ __global__ void __launch_bounds__(D / 2 < 32 ? 32 : D / 2) k_attn_paged_join(con
     T += __shfl_xor_sync(0xffffffffu, T, o);
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
-  if ((threadIdx.x & 31) == 0) {
-    red[0][threadIdx.x >> 5] = T;
-    red[1][threadIdx.x >> 5] = before;
-  }
-  __syncthreads();
-  T = before = 0;
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {
-    T += red[0][w];
-    before += red[1][w];
-  }
-  const int n_units = paged_units(paged_length(p, b));
-  const int d = threadIdx.x * 2;
-  __nv_bfloat16* dst = p.out + static_cast<long long>(b) * p.ldo + static_cast<long long>(head) * D + d;
+  const int n_units = paged_units(p, paged_length(p, b));
+  __nv_bfloat16* dst = p.out + static_cast<long long>(b) * p.ldo + static_cast<long long>(head) * D;
   float* lse = p.lse == nullptr ? nullptr : p.lse + static_cast<long long>(b) * p.heads + head;
   if (n_units == 0) {
-    *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(0.f, 0.f);
-    if (lse != nullptr && d == 0) *lse = -INFINITY;
+    for (int d = threadIdx.x; d < D; d += kPagedJoinWarps * 32) dst[d] = __float2bfloat16_rn(0.f);
+    if (lse != nullptr && threadIdx.x == 0) *lse = -INFINITY;
     return;
   }
   const long long G = paged_ranges(T, ctas);
-  const long long u0 = before + (static_cast<long long>(kvh) * p.chunks + chunk) * n_units;
+  const int kv_group = kvh >> p.team_shift, of = kvh & ((1 << p.team_shift) - 1);
+  const long long u0 = before + (static_cast<long long>(kv_group) * p.chunks + chunk) * n_units;
   const int c0 = paged_owner(u0, T, G), c1 = paged_owner(u0 + n_units - 1, T, G);
   if (c0 == c1) return;  // finished by its CTA
-  auto part = [&](int c) { return p.ws + (2ll * c + (c == c0 ? 1 : 0)) * paged_part_floats<D>(); };
-  float m = -INFINITY;
-  for (int c = c0; c <= c1; ++c) m = fmaxf(m, part(c)[row]);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  float2 acc = make_float2(0.f, 0.f);
-  for (int c = c0; c <= c1; ++c) {
-    const float* w = part(c);
-    const float f = ex2_approx(w[row] - base);
-    l = fmaf(w[kPagedRows + row], f, l);
-    const float2 v = *reinterpret_cast<const float2*>(w + 2 * kPagedRows + row * D + d);
-    acc.x = fmaf(v.x, f, acc.x);
-    acc.y = fmaf(v.y, f, acc.y);
+  float m = -INFINITY, l = 0.f, acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += kPagedJoinWarps) {
+    const float* w = p.ws + (((2ll * c + (c == c0 ? 1 : 0)) << p.team_shift) + of) * paged_part_floats<D>();
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = w[2 * kPagedRows + row * D + 32 * i + lane];
+    const float pm = w[row], pl = w[kPagedRows + row];
+    const float nm = fmaxf(m, pm), base = nm == -INFINITY ? 0.f : nm;
+    const float f0 = ex2_approx(m - base), f1 = ex2_approx(pm - base);
+    m = nm;
+    l = l * f0 + pl * f1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = acc[i] * f0 + v[i] * f1;
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-  if (lse != nullptr && d == 0) *lse = (m + log2f(l)) * 0.69314718055994531f;
+  if (lane == 0) {
+    sm_m[warp] = m;
+    sm_l[warp] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) sm_o[warp][32 * i + lane] = acc[i];
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += kPagedJoinWarps * 32) {
+    float top = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kPagedJoinWarps; ++w) top = fmaxf(top, sm_m[w]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < kPagedJoinWarps; ++w) {
+      const float f = ex2_approx(sm_m[w] - base);
+      sum = fmaf(sm_l[w], f, sum);
+      o = fmaf(sm_o[w][d], f, o);
+    }
+    dst[d] = __float2bfloat16_rn(sum > 0.f ? o / sum : 0.f);
+    if (lse != nullptr && d == 0) *lse = (top + log2f(sum)) * 0.69314718055994531f;
+  }
 }
 
 }  // namespace qib

@@ -115,19 +115,26 @@ static int launch_packed(const void* q, long long ldq, const void* k, long long 
   return launched(launch_pdl(k_attn_packed_join<D>, dim3(grid, 8), dim3(256), 0, stream, 1, p, grid));
 }
 
+// log2 of the most key heads an item may hold: up to 8, evenly.
+static int paged_most_teams(int kv_heads) {
+  int s = 0;
+  while (s < 3 && kv_heads % (2 << s) == 0) ++s;
+  return s;
+}
+
+template <int D, bool FP8, int HT>
+static int launch_paged_tiles(const PagedParams& p, int G, cudaStream_t stream) {
+  constexpr int smem = paged_smem<D, FP8, HT>();
+  if (int rc = allow_smem<&k_attn_paged<D, FP8, HT>>(smem)) return rc;
+  return launched(
+      launch_pdl(k_attn_paged<D, FP8, HT>, dim3(G), dim3(PagedCfg<D, FP8>::THREADS), smem, stream, 1, p));
+}
+
 template <int D, bool FP8>
 static int launch_paged(const PagedParams& p, int G, cudaStream_t stream) {
-  using C = PagedCfg<D, FP8>;
-  int rc;
-  if (p.group <= 8) {
-    if ((rc = allow_smem<&k_attn_paged<D, FP8, true>>(C::SMEM))) return rc;
-    rc = launched(launch_pdl(k_attn_paged<D, FP8, true>, dim3(G), dim3(C::THREADS), C::SMEM, stream, 1, p));
-  } else {
-    if ((rc = allow_smem<&k_attn_paged<D, FP8, false>>(C::SMEM))) return rc;
-    rc = launched(launch_pdl(k_attn_paged<D, FP8, false>, dim3(G), dim3(C::THREADS), C::SMEM, stream, 1, p));
-  }
+  int rc = p.group <= 8 ? launch_paged_tiles<D, FP8, 1>(p, G, stream) : launch_paged_tiles<D, FP8, 2>(p, G, stream);
   if (rc) return rc;
-  return launched(launch_pdl(k_attn_paged_join<D>, dim3(p.heads, p.B), dim3(D / 2), 0, stream, 1, p, G));
+  return launched(launch_pdl(k_attn_paged_join<D>, dim3(p.heads, p.B), dim3(kPagedJoinWarps * 32), 0, stream, 1, p, G));
 }
 
 }  // namespace qib
@@ -299,12 +306,12 @@ int qi_b200_attention_packed_workspace_bytes(int n_seq, int total_q, int total_k
   return QI_B200_OK;
 }
 
-int qi_b200_attention_paged_workspace_bytes(int head_dim, size_t* bytes) {
+int qi_b200_attention_paged_workspace_bytes(int kv_heads, int head_dim, size_t* bytes) {
   if (bytes == nullptr) return QI_B200_EINVAL;
-  if (head_dim != 64 && head_dim != 128) return QI_B200_ESHAPE;
+  if ((head_dim != 64 && head_dim != 128) || kv_heads <= 0) return QI_B200_ESHAPE;
   DeviceInfo* di = nullptr;
   if (int rc = device_info(&di)) return rc;
-  *bytes = static_cast<size_t>(di->num_sms) * 2 *
+  *bytes = (static_cast<size_t>(di->num_sms) * 2 << paged_most_teams(kv_heads)) *
            (head_dim == 128 ? paged_part_floats<128>() : paged_part_floats<64>()) * sizeof(float);
   return QI_B200_OK;
 }
@@ -329,7 +336,7 @@ int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_ca
   DeviceInfo* di = nullptr;
   if (int rc = device_info(&di)) return rc;
   size_t need = 0;
-  if (int rc = qi_b200_attention_paged_workspace_bytes(head_dim, &need)) return rc;
+  if (int rc = qi_b200_attention_paged_workspace_bytes(kv_heads, head_dim, &need)) return rc;
   if (workspace_bytes < need) return QI_B200_EINVAL;
   PagedParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
@@ -357,10 +364,23 @@ int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_ca
   p.group = heads / kv_heads;
   p.chunks = (p.group + kPagedRows - 1) / kPagedRows;
   p.page_size = cache->page_size;
+  p.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (cache->page_size == 1 << s) p.page_shift = s;
   p.max_pages = max_pages;
   p.num_pages = cache->pages;
   p.scale_log2e = scale * 1.4426950408889634f;
   const int G = di->num_sms;
+  // key heads per item: as many as lie next to each other (see the kernel), as
+  // long as the longest the lengths may be still gives every SM four units
+  for (p.team_shift = paged_most_teams(kv_heads); p.team_shift > 0; --p.team_shift) {
+    const long long unit = std::max(16, kPagedUnit >> p.team_shift);
+    const long long tokens = static_cast<long long>(max_pages) * cache->page_size;
+    if (cache->head_stride[0] == head_dim && cache->head_stride[1] == head_dim &&
+        B * ((tokens + unit - 1) / unit) * (kv_heads >> p.team_shift) >= 4ll * G)
+      break;
+  }
+  p.groups = kv_heads >> p.team_shift;
   if (head_dim == 128)
     return cache->fp8 ? launch_paged<128, true>(p, G, stream) : launch_paged<128, false>(p, G, stream);
   return cache->fp8 ? launch_paged<64, true>(p, G, stream) : launch_paged<64, false>(p, G, stream);

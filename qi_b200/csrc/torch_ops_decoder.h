@@ -309,7 +309,7 @@ inline at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_cache
   const c10::cuda::CUDAGuard guard(same.dev);
   at::Tensor o = given(out) ? *out : at::empty({B, heads * D}, q.options());
   size_t ws_bytes = 0;
-  done(qi_b200_attention_paged_workspace_bytes(static_cast<int>(D), &ws_bytes),
+  done(qi_b200_attention_paged_workspace_bytes(small(kv_heads, "kv_heads"), static_cast<int>(D), &ws_bytes),
        "qi_b200_attention_paged_workspace_bytes");
   const at::Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
   done(qi_b200_attention_paged(ptr(q), ldq, &cache, static_cast<const int*>(ptr(pages)),

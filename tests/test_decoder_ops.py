@@ -201,8 +201,8 @@ def test_c_abi_refuses_before_it_touches_the_device():
     assert paged_(q=p + 8) == paged_(ws=p + 8) == _lib.EALIGN
     assert paged_(mp=1 << 28, ld=1 << 28) == _lib.ETOOBIG  # lengths of 2^32 tokens
     assert paged_() == _lib.ECUDA
-    assert lib.qi_b200_attention_paged_workspace_bytes(96, ref(ctypes.c_size_t())) == _lib.ESHAPE
-    assert lib.qi_b200_attention_paged_workspace_bytes(128, None) == _lib.EINVAL
+    assert lib.qi_b200_attention_paged_workspace_bytes(1, 96, ref(ctypes.c_size_t())) == _lib.ESHAPE
+    assert lib.qi_b200_attention_paged_workspace_bytes(1, 128, None) == _lib.EINVAL
 
 
 def test_device_error_names_bad_indexes():

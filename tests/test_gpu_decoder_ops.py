@@ -451,6 +451,8 @@ def paged_ref(q, kc, vc, table, lens, ks, vs, scale, kind):
     ([20000, 1], 4, 2, 32, "token"),          # split over many SMs
     ([37] * 300, 4, 4, 16, "token"),          # many short sequences
     ([0, 0], 2, 1, 16, "token"),
+    ([4000, 1, 0, 2500, 77], 8, 8, 16, "token"),   # all key heads in one item
+    ([3000, 900] * 3, 24, 12, 48, "token"),        # four key heads per item, pages of any size
 ])
 def test_attention_paged(kind, D, lens, hq, hk, page, layout):
     g = gen(sum(lens) + D + hq)
