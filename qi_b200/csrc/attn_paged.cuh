@@ -54,7 +54,7 @@
 namespace qib {
 
 constexpr unsigned int kTagPaged = 0x800u;
-constexpr int kPagedUnit = 64;      // tokens per unit of work, times key heads per item
+constexpr int kPagedUnitShift = 6;  // log2 of tokens per unit of work times key heads per item (16 tokens at least)
 constexpr int kPagedRows = 16;      // query heads per item
 constexpr int kPagedWarps = 8;
 
@@ -74,6 +74,7 @@ struct PagedParams {
   int scale_per_head[2];
   int B, heads, kv_heads, group, chunks;   // chunks of kPagedRows query heads per key head
   int team_shift, groups;                  // log2 of the key heads per item; kv_heads in such groups
+  int unit_shift;                          // log2 of the tokens per unit of work
   int page_size, max_pages, num_pages;
   int page_shift;                          // log2 of page_size, or -1
   float scale_log2e;
@@ -92,10 +93,17 @@ __device__ __forceinline__ int paged_length(const PagedParams& p, int b) {
   }
   return n < 0 ? 0 : n;
 }
-__device__ __forceinline__ int paged_unit(const PagedParams& p) { return max(16, kPagedUnit >> p.team_shift); }
+// Tokens per unit: 2^unit_shift.
 __device__ __forceinline__ int paged_units(const PagedParams& p, int len) {
-  const int n = paged_unit(p);
-  return (len + n - 1) / n;
+  return static_cast<int>((static_cast<long long>(len) + (1 << p.unit_shift) - 1) >> p.unit_shift);
+}
+// The item that a CTA begins and later ones go on with, up to CTA `last`.
+struct PagedRecord {
+  int used, b, kv_group, chunk, last;
+};
+template <int D>
+__device__ __forceinline__ PagedRecord* paged_records(const PagedParams& p, int ctas) {
+  return reinterpret_cast<PagedRecord*>(p.ws + ((2ll * ctas) << p.team_shift) * paged_part_floats<D>());
 }
 
 // Ranges that T units are cut into: none of them is empty, so the partial
@@ -198,6 +206,17 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
   griddep_wait();
   griddep_launch_dependents();
 
+  PagedRecord* rec = paged_records<D>(p, gridDim.x) + blockIdx.x;
+  if (tid == 0) rec->used = 0;
+  // zeros for sequences without keys
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x)
+    if (paged_length(p, b) == 0) {
+      for (int i = tid; i < p.heads * D; i += C::THREADS)
+        p.out[static_cast<long long>(b) * p.ldo + i] = __float2bfloat16_rn(0.f);
+      if (p.lse != nullptr)
+        for (int i = tid; i < p.heads; i += C::THREADS) p.lse[static_cast<long long>(b) * p.heads + i] = -INFINITY;
+    }
+
   // the range of this CTA and the sequence it starts in
   const long long per_unit = static_cast<long long>(p.groups) * p.chunks;
   const int per_thread = (p.B + C::THREADS - 1) / C::THREADS;
@@ -258,7 +277,8 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
     const int unit1 = static_cast<int>(min(static_cast<long long>(n_units), unit0 + (u_end - u)));
     const int kv_group = item / p.chunks, chunk = item - kv_group * p.chunks;
     const int rows = min(kPagedRows, p.group - chunk * kPagedRows);
-    const int tok0 = unit0 * paged_unit(p), tok1 = min(len, unit1 * paged_unit(p));
+    const int tok0 = unit0 << p.unit_shift;
+    const int tok1 = static_cast<int>(min(static_cast<long long>(len), static_cast<long long>(unit1) << p.unit_shift));
     u += unit1 - unit0;
     // this warp's key head, and the blocks of its team: tok0 + (mate + i * mates) * BT
     const int team = warp & ((1 << p.team_shift) - 1), mate = warp >> p.team_shift, mates = W >> p.team_shift;
@@ -529,6 +549,8 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
       }
     __syncthreads();
     const bool whole = unit0 == 0 && unit1 == n_units;
+    if (tid == 0 && unit0 == 0 && !whole)
+      *rec = {1, b, kv_group, chunk, paged_owner(b_first + static_cast<long long>(item + 1) * n_units - 1, T, G)};
     float* parts = p.ws + ((2ll * blockIdx.x + (unit0 == 0 ? 1 : 0)) << p.team_shift) * paged_part_floats<D>();
     for (int i = tid; i < (rows * (D / 2)) << p.team_shift; i += C::THREADS) {
       const int r = i / (D / 2), d = (i - r * (D / 2)) * 2;
@@ -566,69 +588,48 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
   }
 }
 
-// Adds up the partial results of the items that were cut, and writes the rows
-// of sequences without keys (zeros).  One CTA per (sequence, query head); its
-// warps take the parts in turn (a lane D / 32 columns, the maximum in use as
-// above) and add their sums up in warp order.  ctas is the first kernel's grid.
-constexpr int kPagedJoinWarps = 8;
+// Adds up the partial results of the items that were cut: CTA (c, y) query
+// head y of the item that CTA c of the first kernel began and did not finish.
+// Its warps take the parts in turn, four loads ahead, and add their sums up in
+// warp order; a lane holds D / 32 columns.
+constexpr int kPagedJoinWarps = 4;
 template <int D>
 __global__ void __launch_bounds__(kPagedJoinWarps * 32) k_attn_paged_join(const PagedParams p, int ctas) {
   constexpr int N = D / 32;
   __shared__ float sm_m[kPagedJoinWarps], sm_l[kPagedJoinWarps], sm_o[kPagedJoinWarps][D];
   griddep_wait();
   griddep_launch_dependents();
-  const int b = blockIdx.y, head = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int kvh = head / p.group, in_group = head - kvh * p.group;
-  const int chunk = in_group / kPagedRows, row = in_group - chunk * kPagedRows;
-  const long long per_unit = static_cast<long long>(p.groups) * p.chunks;
-  long long before = 0, T = 0;
-  for (int i = lane; i < p.B; i += 32) {  // every warp for itself: no barrier
-    const long long n = paged_units(p, paged_length(p, i)) * per_unit;
-    T += n;
-    if (i < b) before += n;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    T += __shfl_xor_sync(0xffffffffu, T, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
-  const int n_units = paged_units(p, paged_length(p, b));
-  __nv_bfloat16* dst = p.out + static_cast<long long>(b) * p.ldo + static_cast<long long>(head) * D;
-  float* lse = p.lse == nullptr ? nullptr : p.lse + static_cast<long long>(b) * p.heads + head;
-  if (n_units == 0) {
-    for (int d = threadIdx.x; d < D; d += kPagedJoinWarps * 32) dst[d] = __float2bfloat16_rn(0.f);
-    if (lse != nullptr && threadIdx.x == 0) *lse = -INFINITY;
-    return;
-  }
-  const long long G = paged_ranges(T, ctas);
-  const int kv_group = kvh >> p.team_shift, of = kvh & ((1 << p.team_shift) - 1);
-  const long long u0 = before + (static_cast<long long>(kv_group) * p.chunks + chunk) * n_units;
-  const int c0 = paged_owner(u0, T, G), c1 = paged_owner(u0 + n_units - 1, T, G);
-  if (c0 == c1) return;  // finished by its CTA
+  const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const PagedRecord r = paged_records<D>(p, ctas)[c0];
+  if (!r.used) return;
+  const int rows = min(kPagedRows, p.group - r.chunk * kPagedRows);
+  const int of = blockIdx.y / rows, row = blockIdx.y - of * rows;  // key head of the group, query head of its chunk
+  if (of >> p.team_shift) return;
   float m = -INFINITY, l = 0.f, acc[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  for (int k = 0; k < N; ++k) acc[k] = 0.f;
 #pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += kPagedJoinWarps) {
+  for (int c = c0 + warp; c <= r.last; c += kPagedJoinWarps) {
     const float* w = p.ws + (((2ll * c + (c == c0 ? 1 : 0)) << p.team_shift) + of) * paged_part_floats<D>();
     float v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = w[2 * kPagedRows + row * D + 32 * i + lane];
+    for (int k = 0; k < N; ++k) v[k] = w[2 * kPagedRows + row * D + 32 * k + lane];
     const float pm = w[row], pl = w[kPagedRows + row];
     const float nm = fmaxf(m, pm), base = nm == -INFINITY ? 0.f : nm;
     const float f0 = ex2_approx(m - base), f1 = ex2_approx(pm - base);
     m = nm;
     l = l * f0 + pl * f1;
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = acc[i] * f0 + v[i] * f1;
+    for (int k = 0; k < N; ++k) acc[k] = acc[k] * f0 + v[k] * f1;
   }
   if (lane == 0) {
     sm_m[warp] = m;
     sm_l[warp] = l;
   }
 #pragma unroll
-  for (int i = 0; i < N; ++i) sm_o[warp][32 * i + lane] = acc[i];
+  for (int k = 0; k < N; ++k) sm_o[warp][32 * k + lane] = acc[k];
   __syncthreads();
+  const int head = ((r.kv_group << p.team_shift) + of) * p.group + r.chunk * kPagedRows + row;
   for (int d = threadIdx.x; d < D; d += kPagedJoinWarps * 32) {
     float top = -INFINITY, sum = 0.f, o = 0.f;
 #pragma unroll
@@ -640,8 +641,10 @@ __global__ void __launch_bounds__(kPagedJoinWarps * 32) k_attn_paged_join(const 
       sum = fmaf(sm_l[w], f, sum);
       o = fmaf(sm_o[w][d], f, o);
     }
-    dst[d] = __float2bfloat16_rn(sum > 0.f ? o / sum : 0.f);
-    if (lse != nullptr && d == 0) *lse = (top + log2f(sum)) * 0.69314718055994531f;
+    p.out[static_cast<long long>(r.b) * p.ldo + static_cast<long long>(head) * D + d] =
+        __float2bfloat16_rn(sum > 0.f ? o / sum : 0.f);
+    if (p.lse != nullptr && d == 0)
+      p.lse[static_cast<long long>(r.b) * p.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
   }
 }
 

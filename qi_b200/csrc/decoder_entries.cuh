@@ -134,7 +134,9 @@ template <int D, bool FP8>
 static int launch_paged(const PagedParams& p, int G, cudaStream_t stream) {
   int rc = p.group <= 8 ? launch_paged_tiles<D, FP8, 1>(p, G, stream) : launch_paged_tiles<D, FP8, 2>(p, G, stream);
   if (rc) return rc;
-  return launched(launch_pdl(k_attn_paged_join<D>, dim3(p.heads, p.B), dim3(kPagedJoinWarps * 32), 0, stream, 1, p, G));
+  const int heads = std::min(kPagedRows, p.group) << p.team_shift;  // query heads of an item
+  return launched(
+      launch_pdl(k_attn_paged_join<D>, dim3(G, heads), dim3(kPagedJoinWarps * 32), 0, stream, 1, p, G));
 }
 
 }  // namespace qib
@@ -312,7 +314,8 @@ int qi_b200_attention_paged_workspace_bytes(int kv_heads, int head_dim, size_t* 
   DeviceInfo* di = nullptr;
   if (int rc = device_info(&di)) return rc;
   *bytes = (static_cast<size_t>(di->num_sms) * 2 << paged_most_teams(kv_heads)) *
-           (head_dim == 128 ? paged_part_floats<128>() : paged_part_floats<64>()) * sizeof(float);
+               (head_dim == 128 ? paged_part_floats<128>() : paged_part_floats<64>()) * sizeof(float) +
+           di->num_sms * sizeof(PagedRecord);
   return QI_B200_OK;
 }
 
@@ -374,13 +377,14 @@ int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_ca
   // key heads per item: as many as lie next to each other (see the kernel), as
   // long as the longest the lengths may be still gives every SM four units
   for (p.team_shift = paged_most_teams(kv_heads); p.team_shift > 0; --p.team_shift) {
-    const long long unit = std::max(16, kPagedUnit >> p.team_shift);
+    const long long unit = 1ll << std::max(4, kPagedUnitShift - p.team_shift);
     const long long tokens = static_cast<long long>(max_pages) * cache->page_size;
     if (cache->head_stride[0] == head_dim && cache->head_stride[1] == head_dim &&
         B * ((tokens + unit - 1) / unit) * (kv_heads >> p.team_shift) >= 4ll * G)
       break;
   }
   p.groups = kv_heads >> p.team_shift;
+  p.unit_shift = std::max(4, kPagedUnitShift - p.team_shift);
   if (head_dim == 128)
     return cache->fp8 ? launch_paged<128, true>(p, G, stream) : launch_paged<128, false>(p, G, stream);
   return cache->fp8 ? launch_paged<64, true>(p, G, stream) : launch_paged<64, false>(p, G, stream);
