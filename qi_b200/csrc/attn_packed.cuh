@@ -162,37 +162,46 @@ __device__ __forceinline__ void packed_span(const int* cu, int b, int total, int
   len = min(max(cu[b + 1], first), total) - first;
 }
 
-// The 128-key steps of the two tiles of an item (query block `level` of sequence b).
-struct PackedGeometry {
-  int q0, lq, k0, lk, n[2];
+// First rows and lengths of a sequence (zeros behind the last one).
+struct PackedSpan {
+  int q0, lq, k0, lk;
 };
-__device__ __forceinline__ PackedGeometry packed_geometry(const PackedParams& p, int b, int level) {
-  PackedGeometry g;
-  packed_span(p.cu_q, b, p.total_q, g.q0, g.lq);
-  packed_span(p.cu_k, b, p.total_k, g.k0, g.lk);
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int m = p.pair_heads ? level * 128 : level * 256 + 128 * t;
-    const int rows = min(128, g.lq - m);
-    const int visible = p.causal ? min(g.lk, m + rows + g.lk - g.lq) : g.lk;
-    g.n[t] = rows > 0 && visible > 0 ? (visible + 127) / 128 : 0;
+__device__ __forceinline__ PackedSpan packed_load(const PackedParams& p, int b) {
+  PackedSpan s = {0, 0, 0, 0};
+  if (b < p.n_seq) {
+    packed_span(p.cu_q, b, p.total_q, s.q0, s.lq);
+    packed_span(p.cu_k, b, p.total_k, s.k0, s.lk);
   }
-  return g;
+  return s;
+}
+__device__ __forceinline__ PackedSpan packed_from_lane(const PackedSpan& s, int lane) {
+  return {__shfl_sync(0xffffffffu, s.q0, lane), __shfl_sync(0xffffffffu, s.lq, lane),
+          __shfl_sync(0xffffffffu, s.k0, lane), __shfl_sync(0xffffffffu, s.lk, lane)};
+}
+// 128-key steps of tile t of query block `level`.
+__device__ __forceinline__ int packed_tile_steps(const PackedParams& p, const PackedSpan& s, int level, int t) {
+  const int m = p.pair_heads ? level * 128 : level * 256 + 128 * t;
+  const int rows = min(128, s.lq - m);
+  const int visible = p.causal ? min(s.lk, m + rows + s.lk - s.lq) : s.lk;
+  return rows > 0 && visible > 0 ? (visible + 127) / 128 : 0;
+}
+__device__ __forceinline__ int packed_steps(const PackedParams& p, const PackedSpan& s, int level) {
+  return max(packed_tile_steps(p, s, level, 0), packed_tile_steps(p, s, level, 1));
 }
 
 // Steps [lo, hi) of an item (counted from its first key); whole where that is all of it.
-__device__ __forceinline__ PackedItem packed_item(const PackedParams& p, const PackedGeometry& g, int level, int hi_,
+__device__ __forceinline__ PackedItem packed_item(const PackedParams& p, const PackedSpan& s, int level, int hi_,
                                                   int lo, int hi, int part) {
   PackedItem it;
-  it.q0 = g.q0, it.lq = g.lq;
-  it.k0 = g.k0 + lo * 128, it.lk = g.lk - lo * 128;
+  it.q0 = s.q0, it.lq = s.lq;
+  it.k0 = s.k0 + lo * 128, it.lk = s.lk - lo * 128;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     it.head[t] = p.pair_heads ? 2 * hi_ + t : hi_;
     it.m[t] = p.pair_heads ? level * 128 : level * 256 + 128 * t;
-    it.n[t] = max(0, min(g.n[t], hi) - lo);
+    it.n[t] = max(0, min(packed_tile_steps(p, s, level, t), hi) - lo);
   }
-  it.diag = p.causal ? it.lk - it.lq : 0x3fffffff - g.lq;
+  it.diag = p.causal ? it.lk - it.lq : 0x3fffffff - s.lq;
   it.part = part;
   it.last = 0;
   return it;
@@ -209,13 +218,17 @@ struct PackedRecord {
   int row[2], rows[2], head[2];
 };
 
+// What an item costs beside its steps, in steps (measured: 4 us for an item of
+// one step, 1.8 us for every further one).
+constexpr int kPackedItemCost = 2;
+
 // An even split pays where the longest-first order leaves SMs idle for longer
 // than writing and joining the partial results takes (about 12 us, 7 steps).
 // What that order leaves idle: at most one item per CTA, the longest; equal
 // items, what the last round lacks; falling lengths, about half the length of
 // the last round's items.
-__device__ __forceinline__ bool packed_even_split(long long steps, long long items, int longest, int G, int causal) {
-  const long long even = steps / G;
+__device__ __forceinline__ bool packed_even_split(long long cost, long long items, int longest, int G, int causal) {
+  const long long even = cost / G;
   long long order;
   if (items <= G) order = longest;
   else if (!causal) order = (items + G - 1) / G * longest;
@@ -224,40 +237,46 @@ __device__ __forceinline__ bool packed_even_split(long long steps, long long ite
 }
 
 // The items of this CTA one after another to `put` (the whole warp calls it).
+// A lane holds the span of a sequence, 32 sequences at a time.
 template <int D, class Put>
 __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) {
   const int lane = threadIdx.x & 31;
-  const int rows_per_item = p.pair_heads ? 128 : 256;
+  const int block_shift = p.pair_heads ? 7 : 8;  // query rows per item
   const int heads_items = p.pair_heads ? p.heads / 2 : p.heads;
   const int G = gridDim.x, me = blockIdx.x;
-  auto blocks = [&](int b) {
-    if (b >= p.n_seq) return 0;
-    int first, len;
-    packed_span(p.cu_q, b, p.total_q, first, len);
-    return (len + rows_per_item - 1) / rows_per_item;
+  PackedSpan span = packed_load(p, lane);
+  auto blocks = [&](const PackedSpan& s) { return (s.lq + (1 << block_shift) - 1) >> block_shift; };
+  auto end_of_items = [&]() {
+    PackedItem end = {};
+    end.last = 1;
+    put(end);
   };
-  auto steps_of = [&](int b, int level) {
-    const PackedGeometry g = packed_geometry(p, b, level);
-    return max(g.n[0], g.n[1]);
+  int most = 0, longest = 0, count = 0;
+  long long total = 0;
+  auto seq_cost = [&](const PackedSpan& s) {  // cost of one head item of each block with keys
+    const int nb = blocks(s);
+    int sum = 0;
+    for (int level = 0; level < nb; ++level) {
+      const int n = packed_steps(p, s, level);
+      sum += n + (n > 0 ? kPackedItemCost : 0);
+      longest = max(longest, n + kPackedItemCost);
+    }
+    return sum;
   };
+  for (int chunk = 0; chunk < p.n_seq; chunk += 32) {
+    const PackedSpan s = chunk ? packed_load(p, chunk + lane) : span;
+    most = max(most, blocks(s));
+    if (p.ws != nullptr) {
+      total += seq_cost(s);
+      count += blocks(s);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
   if (p.ws != nullptr) {
     PackedRecord* rec = reinterpret_cast<PackedRecord*>(p.ws + 2ll * G * packed_part_floats<D>()) + 2 * me;
     if (lane < 2) rec[lane].used = 0;
     __syncwarp();
-    long long total = 0;
-    int longest = 0, count = 0;
-    auto seq_steps = [&](int b) {  // steps of one head item of sequence b
-      const int nb = blocks(b);
-      int sum = 0;
-      for (int level = 0; level < nb; ++level) {
-        const int s = steps_of(b, level);
-        sum += s;
-        longest = max(longest, s);
-      }
-      count += nb;
-      return sum;
-    };
-    for (int b = lane; b < p.n_seq; b += 32) total += seq_steps(b);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -266,10 +285,11 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
     }
     total *= heads_items;
     if (packed_even_split(total, static_cast<long long>(count) * heads_items, longest, G, p.causal)) {
-      // the steps of all items end to end (sequences in order, blocks in order,
-      // heads), cut into equal ranges of three steps or more, so that the parts of
-      // an item are those of consecutive CTAs; an item's last steps come first in it
-      const long long cuts = max(1ll, min(static_cast<long long>(G), total / 3));
+      // the costs of all items end to end (sequences in order, blocks in order,
+      // heads; an item's fixed cost, then its steps from the last to the first),
+      // cut into equal ranges long enough for three steps, so that the parts of an
+      // item are those of consecutive CTAs
+      const long long cuts = max(1ll, min(static_cast<long long>(G), total / (kPackedItemCost + 3)));
       const long long lo = total * min(static_cast<long long>(me), cuts) / cuts;
       const long long hi = total * min(me + 1ll, cuts) / cuts;
       auto scan = [&](long long v) {  // inclusive, over the lanes
@@ -280,39 +300,40 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
         }
         return v;
       };
-      long long before = 0;  // steps of the sequences in front of the chunk
+      auto cost_of = [&](int steps) { return steps > 0 ? (steps + kPackedItemCost) * static_cast<long long>(heads_items) : 0; };
+      long long before = 0;  // cost of the sequences in front of the chunk
       int idle = 0;          // blocks without steps so far (zeros to write: the CTAs take turns at them)
       for (int chunk = 0; chunk < p.n_seq; chunk += 32) {
-        const long long mine = static_cast<long long>(seq_steps(chunk + lane)) * heads_items;
+        if (chunk) span = packed_load(p, chunk + lane);
+        const long long mine = static_cast<long long>(seq_cost(span)) * heads_items;
         const long long end = before + scan(mine);
         unsigned todo = __ballot_sync(0xffffffffu, end > lo && end - mine < hi && mine > 0);
         while (todo) {
           const int i = __ffs(todo) - 1;
           todo &= todo - 1;
-          const int b = chunk + i, nb = blocks(b);
+          const PackedSpan s = packed_from_lane(span, i);
+          const int nb = blocks(s);
           long long at = __shfl_sync(0xffffffffu, end - mine, i);
           for (int l0 = 0; l0 < nb && at < hi; l0 += 32) {
-            const int s_lane = l0 + lane < nb ? steps_of(b, l0 + lane) : 0;
-            const long long l_end = at + scan(static_cast<long long>(s_lane) * heads_items);
-            unsigned levels = __ballot_sync(0xffffffffu, s_lane > 0 && l_end > lo &&
-                                                             l_end - static_cast<long long>(s_lane) * heads_items < hi);
+            const int s_lane = l0 + lane < nb ? packed_steps(p, s, l0 + lane) : 0;
+            const long long l_end = at + scan(cost_of(s_lane));
+            unsigned levels = __ballot_sync(0xffffffffu, s_lane > 0 && l_end > lo && l_end - cost_of(s_lane) < hi);
             while (levels) {
               const int j = __ffs(levels) - 1;
               levels &= levels - 1;
-              const int level = l0 + j;
-              const PackedGeometry g = packed_geometry(p, b, level);
-              const int s = max(g.n[0], g.n[1]);
-              const long long first = __shfl_sync(0xffffffffu, l_end, j) - static_cast<long long>(s) * heads_items;
-              int h = first < lo ? static_cast<int>((lo - first) / s) : 0;
-              for (long long u = first + static_cast<long long>(h) * s; h < heads_items && u < hi; ++h, u += s) {
-                const int from = static_cast<int>(max(0ll, lo - u));
-                const int to = static_cast<int>(min(static_cast<long long>(s), hi - u));
-                const int part = from == 0 && to == s ? -1 : (from == 0 ? 1 : 0);
-                const PackedItem it = packed_item(p, g, level, h, s - to, s - from, part);
+              const int n = __shfl_sync(0xffffffffu, s_lane, j), per = n + kPackedItemCost;
+              const long long first = __shfl_sync(0xffffffffu, l_end, j) - cost_of(n);
+              int h = first < lo ? static_cast<int>((lo - first) / per) : 0;
+              for (long long u = first + static_cast<long long>(h) * per; h < heads_items && u < hi; ++h, u += per) {
+                const int from = static_cast<int>(max(0ll, lo - u - kPackedItemCost));
+                const int to = static_cast<int>(max(0ll, min(static_cast<long long>(n), hi - u - kPackedItemCost)));
+                if (from >= to) continue;
+                const int part = from == 0 && to == n ? -1 : (from == 0 ? 1 : 0);
+                const PackedItem it = packed_item(p, s, l0 + j, h, n - to, n - from, part);
                 if (part >= 0 && lane == 0) {
                   PackedRecord r;
                   r.used = 1;
-                  r.ends = to == s;
+                  r.ends = to == n;
 #pragma unroll
                   for (int t = 0; t < 2; ++t) {
                     r.row[t] = it.q0 + it.m[t];
@@ -329,37 +350,31 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
         }
         before = __shfl_sync(0xffffffffu, end, 31);
         int none = 0;
-        for (int level = 0; level < blocks(chunk + lane); ++level) none += steps_of(chunk + lane, level) == 0;
+        for (int level = 0; level < blocks(span); ++level) none += packed_steps(p, span, level) == 0;
         unsigned with = __ballot_sync(0xffffffffu, none > 0);
         while (with) {
           const int i = __ffs(with) - 1;
           with &= with - 1;
-          const int b = chunk + i, nb = blocks(b);
+          const PackedSpan s = packed_from_lane(span, i);
+          const int nb = blocks(s);
           for (int level = 0; level < nb; ++level) {
-            const PackedGeometry g = packed_geometry(p, b, level);
-            if (g.n[0] > 0 || g.n[1] > 0) continue;
+            if (packed_steps(p, s, level) > 0) continue;
             for (int h = (me + idle) % G; h < heads_items; h += G)
-              if (!put(packed_item(p, g, level, h, 0, 0, -1))) return;
+              if (!put(packed_item(p, s, level, h, 0, 0, -1))) return;
             ++idle;
           }
         }
       }
-      PackedItem end = {};
-      end.last = 1;
-      put(end);
+      end_of_items();
       return;
     }
   }
   // longest first: level by level from the last
-  int most = 0;
-  for (int b = lane; b < p.n_seq; b += 32) most = max(most, blocks(b));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-  const int blocks0 = blocks(lane);
   int base = 0, round = 0;  // items before this (level, chunk); rounds of G items begun
   for (int level = most - 1; level >= 0; --level) {
     for (int chunk = 0; chunk < p.n_seq; chunk += 32) {
-      unsigned active = __ballot_sync(0xffffffffu, (chunk == 0 ? blocks0 : blocks(chunk + lane)) > level);
+      if (p.n_seq > 32) span = packed_load(p, chunk + lane);
+      const unsigned active = __ballot_sync(0xffffffffu, blocks(span) > level);
       const int n = __popc(active) * heads_items;
       while (true) {
         const int idx = round * G + ((round & 1) ? G - 1 - me : me) - base;
@@ -368,15 +383,13 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
         const int nth = idx / heads_items, hi = idx - nth * heads_items;
         unsigned mm = active;
         for (int i = 0; i < nth; ++i) mm &= mm - 1;
-        const PackedGeometry g = packed_geometry(p, chunk + __ffs(mm) - 1, level);
-        if (!put(packed_item(p, g, level, hi, 0, max(g.n[0], g.n[1]), -1))) return;
+        const PackedSpan s = packed_from_lane(span, __ffs(mm) - 1);
+        if (!put(packed_item(p, s, level, hi, 0, packed_steps(p, s, level), -1))) return;
       }
       base += n;
     }
   }
-  PackedItem end = {};
-  end.last = 1;
-  put(end);
+  end_of_items();
 }
 
 template <int D>
