@@ -12,7 +12,7 @@
 // 176 us with one head at a time, 168 / 162 / 161 with 2 / 4 / 8; E4M3 rows of
 // 128 bytes 151, 126, 121, 115).
 //
-// Split: the work of all items, counted in units of at least 16 tokens, is laid
+// Split: the work of all items, counted in units of 16 tokens or more, is laid
 // end to end and cut into gridDim.x equal ranges, one per CTA, so every SM
 // streams the same number of bytes whatever the lengths are.  An item inside
 // one range is finished there; an item cut by range borders leaves partial
@@ -54,7 +54,7 @@
 namespace qib {
 
 constexpr unsigned int kTagPaged = 0x800u;
-constexpr int kPagedUnitShift = 6;  // log2 of tokens per unit of work times key heads per item (16 tokens at least)
+constexpr int kPagedUnitShift = 6;  // log2 of tokens per unit of work times key heads per item (a block at least)
 constexpr int kPagedRows = 16;      // query heads per item
 constexpr int kPagedWarps = 8;
 
@@ -173,6 +173,7 @@ struct PagedCfg {
   static constexpr int WARPS = kPagedWarps;
   static constexpr int STAGE = ROW == 64 ? 4096 : 8192;
   static constexpr int BT = STAGE / (2 * ROW);              // tokens per block: 16 or 32
+  static_assert(BT == (ROW == 256 ? 16 : 32), "the entry point sizes the units of work by it");
   static constexpr int CH = ROW / 16;                       // 16-byte chunks per row: 4, 8 or 16
   static constexpr int STAGES = 24576 / STAGE;              // 192 KB in all
   static constexpr int THREADS = WARPS * 32;
@@ -260,7 +261,8 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
   long long b_first = start_u;  // first unit of sequence b
   const uint32_t ring_u = smem_u32(paged_sm + warp * ST * C::STAGE);
   const int g = lane >> 2, t4 = lane & 3;
-  const bool whole_pages = p.page_shift >= 0 && (1 << p.page_shift) >= BT;  // blocks start at multiples of BT
+  // a block lies in one page: units, where ranges begin, are multiples of BT
+  const bool whole_pages = p.page_shift >= 0 && (1 << p.page_shift) >= BT && (1 << p.unit_shift) >= BT;
 
   while (u < u_end) {
     int len = paged_length(p, b);

@@ -376,15 +376,18 @@ int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_ca
   const int G = di->num_sms;
   // key heads per item: as many as lie next to each other (see the kernel), as
   // long as the longest the lengths may be still gives every SM four units
+  // a unit holds a whole number of a warp's blocks (16 tokens of 256-byte rows,
+  // else 32), so that blocks keep to multiples of their size and to one page
+  const int block_shift = head_dim * elt == 256 ? 4 : 5;
   for (p.team_shift = paged_most_teams(kv_heads); p.team_shift > 0; --p.team_shift) {
-    const long long unit = 1ll << std::max(4, kPagedUnitShift - p.team_shift);
+    const long long unit = 1ll << std::max(block_shift, kPagedUnitShift - p.team_shift);
     const long long tokens = static_cast<long long>(max_pages) * cache->page_size;
     if (cache->head_stride[0] == head_dim && cache->head_stride[1] == head_dim &&
         B * ((tokens + unit - 1) / unit) * (kv_heads >> p.team_shift) >= 4ll * G)
       break;
   }
   p.groups = kv_heads >> p.team_shift;
-  p.unit_shift = std::max(4, kPagedUnitShift - p.team_shift);
+  p.unit_shift = std::max(block_shift, kPagedUnitShift - p.team_shift);
   if (head_dim == 128)
     return cache->fp8 ? launch_paged<128, true>(p, G, stream) : launch_paged<128, false>(p, G, stream);
   return cache->fp8 ? launch_paged<64, true>(p, G, stream) : launch_paged<64, false>(p, G, stream);

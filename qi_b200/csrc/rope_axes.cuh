@@ -9,7 +9,8 @@
 //
 // Angles: the turn pos * freq / (2 pi) is formed and reduced to [-1/2, 1/2]
 // in 64 bits (an fp32 product is off by up to 2^-24 of the whole angle: 0.06
-// rad at position 10^6), and sin / cos of the reduced turn are taken in fp32.
+// rad at position 10^6), and sin / cos of the reduced turn are taken in fp32,
+// with a first-order step for what the fp32 turn leaves out.
 // They depend on the token and the pair only, so a CTA computes them once for
 // its tokens and every head reads them from shared memory; no table per token
 // exists in memory.
@@ -150,10 +151,14 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_axes(const RopeAxesParams
     else
       record_error(kDevBadIndex, kTagRope, 1);
     turn -= rint(turn);
+    // the half turns as a sum of two floats; sin and cos of the first, turned on by the second
+    const double half = 2.0 * turn;
+    const float hi = static_cast<float>(half);
+    const float lo = static_cast<float>(half - static_cast<double>(hi)) * 3.14159265f;
     float sn, c;
-    sincospif(2.0f * static_cast<float>(turn), &sn, &c);
-    cs[0][i] = c;
-    cs[1][i] = sn;
+    sincospif(hi, &sn, &c);
+    cs[0][i] = fmaf(-sn, lo, c);
+    cs[1][i] = fmaf(c, lo, sn);
   }
   if (CACHE && threadIdx.x < nt) {
     long long s = load_index(p.slots, m0 + threadIdx.x, p.slots64);

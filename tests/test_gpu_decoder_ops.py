@@ -453,6 +453,8 @@ def paged_ref(q, kc, vc, table, lens, ks, vs, scale, kind):
     ([0, 0], 2, 1, 16, "token"),
     ([4000, 1, 0, 2500, 77], 8, 8, 16, "token"),   # all key heads in one item
     ([3000, 900] * 3, 24, 12, 48, "token"),        # four key heads per item, pages of any size
+    ([9000, 5555, 777, 2048], 16, 8, 64, "token"),  # ranges that begin anywhere in a page
+    ([4100, 61, 3333], 4, 4, 32, "token"),
 ])
 def test_attention_paged(kind, D, lens, hq, hk, page, layout):
     g = gen(sum(lens) + D + hq)
