@@ -29,17 +29,21 @@
 // block of every sequence that has one) from the last to the first; warp 10
 // walks it and hands the items over in shared memory, four in flight.
 //
-// What bounds it: the chain of one tile, softmax (about 2,250 clocks, 1,024 of
+// What bounds it: the chain of one tile, softmax (about 2,200 clocks, 1,024 of
 // them exponentials) then P V and S (1,300 clocks, 1,024 of them products),
-// 3,750 clocks per 128-key step where the products of both tiles take 2,048.
-// Measured on the way (16384 tokens, 24 / 8 heads of 128, causal, us): products
-// issued by lane 0 with 64-bit descriptors formed on the spot 1,842, by an
-// elected thread 1,645, item list in a warp of its own and descriptors as
-// constants to a base 1,371, all MMA operands warp-uniform 1,330.  Two threads
+// 3,600 clocks per 128-key step where the products of both tiles take 2,048.
+// Measured on the way (16384 tokens, 24 / 8 heads of 128, causal, us; 1,263 is
+// 1,306 TFLOP/s): products issued by lane 0 with 64-bit descriptors formed on
+// the spot 1,842, by an elected thread 1,645, item list in a warp of its own and
+// descriptors as constants to a base 1,371, all MMA operands warp-uniform 1,330,
+// S loaded in one go 1,297, the masked keys in one branch 1,263.  Two threads
 // per row (16 softmax warps) 1,433; half of P handed over early 1,359; 64-key
 // steps with S double-buffered 1,457 (the products read shared memory at its
 // full rate then, and every barrier waits behind them); a quarter of the
-// exponentials as polynomials on the FP32 pipe 1,365.
+// exponentials as polynomials on the FP32 pipe 1,365; masks by 32-key chunk
+// 1,351 (branches between the loads and the maximum).
+// A short item costs about 4 us beside its further steps: both tiles' softmax
+// fall together, then the output.
 //
 // Rows behind a sequence's end belong to its neighbour: scores of such keys
 // are replaced (not added to), the V rows of the last 16-key step behind the
@@ -504,6 +508,8 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       while (const PackedItem* it = next_item()) {
         const int steps = max(it->n[0], it->n[1]);
         const int q0 = it->q0, k0 = it->k0, col = it->head[0] / p.group * D;
+        // the first K goes ahead of Q, whose places are free later
+        if (steps > 0) load(&tmK, col, k0 + (steps - 1) * 128);
         if (steps > 0) {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
@@ -521,7 +527,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         }
         release_item();
         for (int j = steps - 1; j >= 0 && ok; --j) {
-          load(&tmK, col, k0 + j * 128);
+          if (j < steps - 1) load(&tmK, col, k0 + j * 128);
           load(&tmV, col, k0 + j * 128);
         }
         if (!ok) break;
@@ -662,8 +668,9 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     bool ok = true;
     while (const PackedItem* it = next_item()) {
       const int steps = it->n[t];
-      // last visible key of this row and of the tile's first row
-      const int first_limit = min(it->lk - 1, it->m[t] + it->diag), limit = min(it->lk - 1, it->m[t] + row + it->diag);
+      // last visible key of this row, and of the warp's first
+      const int reach = it->m[t] + (warp & 3) * 32 + it->diag, last_key = it->lk - 1;
+      const int limit = min(last_key, reach + lane), first_limit = min(last_key, reach);
       float m_use = -INFINITY;
       float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       for (int j = steps - 1; j >= 0; --j) {
@@ -673,20 +680,20 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         uint32_t r[4][32];
         tmem_ld_32x32b_x32(t_s, r[0]);
         tmem_ld_32x32b_x32(t_s + 32, r[1]);
-        tmem_ld_wait();
         tmem_ld_32x32b_x32(t_s + 64, r[2]);
         tmem_ld_32x32b_x32(t_s + 96, r[3]);
-        const bool cut = j * 128 + 127 > first_limit;
-        const int lim = limit - j * 128;
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // independent chains
+        tmem_ld_wait();
+        if (j * 128 + 127 > first_limit) {
+          const int lim = limit - j * 128;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c == 2) tmem_ld_wait();
-          if (cut) {
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i > lim) r[c][i] = 0xff800000u;  // -inf
-          }
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // independent chains
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
 #pragma unroll
           for (int i = 0; i < 32; i += 2)
             mx4[(i >> 1) & 3] = fmaxf(mx4[(i >> 1) & 3], fmaxf(__uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1])));
@@ -776,32 +783,44 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       // that neither side has bank conflicts), so that a store covers whole lines;
       // a row per thread would touch 32 lines with each
       uint8_t* box = staging + warp * 4096;
+      // a lane stores chunk lane % 8 of rows lane / 8, lane / 8 + 4, ... (their places alternate between two)
+      const uint8_t* box_even = box + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
+      const uint8_t* box_odd = box + (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) + 4)) << 4);
+      __nv_bfloat16* lane_dst = dst + (lane >> 3) * p.ldo + (lane & 7) * 8;
+      uint32_t o[D / 32][32];
+      if (steps > 0) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) tmem_ld_32x32b_x32(t_o + 32 * c, o[c]);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[c][i] = 0u;
+      }
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t o[32];
-          if (steps > 0) {
-            tmem_ld_32x32b_x32(t_o + 64 * c + 32 * h, o);
-            tmem_ld_wait();
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0u;
-          }
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * i + e]) * inv;
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[2 * c + h][8 * i + e]) * inv;
             *reinterpret_cast<uint4*>(box + lane * 128 + (((4 * h + i) ^ (lane & 7)) << 4)) = pack8(f);
           }
-        }
         __syncwarp();
+        __nv_bfloat16* to = lane_dst + 64 * c;
+        if (rows >= 32) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 4 * i + (lane >> 3);
-          const uint4 v = *reinterpret_cast<const uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-          if (r < rows) *reinterpret_cast<uint4*>(dst + r * p.ldo + 64 * c + (lane & 7) * 8) = v;
+          for (int i = 0; i < 8; ++i, to += 4 * p.ldo)
+            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(i & 1 ? box_odd + i * 512 : box_even + i * 512);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i, to += 4 * p.ldo)
+            if (4 * i + (lane >> 3) < rows)
+              *reinterpret_cast<uint4*>(to) =
+                  *reinterpret_cast<const uint4*>(i & 1 ? box_odd + i * 512 : box_even + i * 512);
         }
         __syncwarp();
       }
