@@ -256,6 +256,7 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
     put(end);
   };
   int most = 0, longest = 0, count = 0;
+  int chunk_most = 0;  // most blocks of a sequence in the lane's chunk of 32 (of the first 32 chunks)
   long long total = 0;
   auto seq_cost = [&](const PackedSpan& s) {  // cost of one head item of each block with keys
     const int nb = blocks(s);
@@ -269,14 +270,14 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
   };
   for (int chunk = 0; chunk < p.n_seq; chunk += 32) {
     const PackedSpan s = chunk ? packed_load(p, chunk + lane) : span;
-    most = max(most, blocks(s));
+    const int chunk_max = __reduce_max_sync(0xffffffffu, blocks(s));
+    most = max(most, chunk_max);
+    if (lane == chunk >> 5) chunk_most = chunk_max;
     if (p.ws != nullptr) {
       total += seq_cost(s);
       count += blocks(s);
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
   if (p.ws != nullptr) {
     PackedRecord* rec = reinterpret_cast<PackedRecord*>(p.ws + 2ll * G * packed_part_floats<D>()) + 2 * me;
     if (lane < 2) rec[lane].used = 0;
@@ -376,7 +377,9 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
   // longest first: level by level from the last
   int base = 0, round = 0;  // items before this (level, chunk); rounds of G items begun
   for (int level = most - 1; level >= 0; --level) {
+    const unsigned with = __ballot_sync(0xffffffffu, chunk_most > level);
     for (int chunk = 0; chunk < p.n_seq; chunk += 32) {
+      if (chunk < 1024 && !((with >> (chunk >> 5)) & 1u)) continue;
       if (p.n_seq > 32) span = packed_load(p, chunk + lane);
       const unsigned active = __ballot_sync(0xffffffffu, blocks(span) > level);
       const int n = __popc(active) * heads_items;

@@ -335,7 +335,7 @@ int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_ca
   if (ldq < wq || ldo < wq || ldq % 8 || ldo % 8) return QI_B200_ESHAPE;
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace)) return QI_B200_EALIGN;
   if (int rc = check_paged_cache(cache, kv_heads, head_dim)) return rc;
-  if (static_cast<long long>(max_pages) * cache->page_size > 0x7fffffffll) return QI_B200_ETOOBIG;
+  if (static_cast<long long>(max_pages) * cache->page_size > 0x7fff0000ll) return QI_B200_ETOOBIG;
   DeviceInfo* di = nullptr;
   if (int rc = device_info(&di)) return rc;
   size_t need = 0;

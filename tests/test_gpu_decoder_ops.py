@@ -243,6 +243,27 @@ def test_rope_axes_store(kind, M, hq, hk, D, page, layout):
         assert (c[r // page, r % page] == 3).all()  # every other slot as it was
 
 
+def test_rope_axes_store_index_and_code_types():
+    """int32 slots and a float8_e4m3fn cache give what int64 slots and a uint8 cache give."""
+    g = gen(2)
+    M, hk, D = 37, 2, 64
+    x = randn(g, M, 3 * hk * D)
+    q, k, v = x.split(hk * D, 1)
+    freqs, axes = K.rope_axes_frequencies((32,), device=DEV)
+    pos = torch.arange(M, device=DEV)
+    slots = torch.randperm(64, generator=g)[:M].to(DEV)
+    s = torch.full((1,), 0.02, device=DEV)
+    out = []
+    for dt, idx in ((torch.uint8, torch.int64), (torch.float8_e4m3fn, torch.int32)):
+        kc, vc = (torch.zeros(8, 8, hk, D, dtype=torch.uint8, device=DEV).view(dt) for _ in range(2))
+        K.rope_axes_store(q, k, v, pos.to(idx), freqs, axes, D, kc, vc, slots.to(idx), k_scale=s, v_scale=s)
+        table, n = torch.arange(8, dtype=torch.int32, device=DEV)[None], torch.tensor([60], dtype=torch.int32, device=DEV)
+        out.append((kc.view(torch.uint8), vc.view(torch.uint8),
+                    K.attention_paged(q[:1], kc, vc, table, n, k_scale=s, v_scale=s)))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+
+
 def test_rope_axes_store_reports_slots_outside_the_cache():
     g = gen(1)
     x = randn(g, 4, 3 * 64)
@@ -333,6 +354,7 @@ PACKED = [
     ([700, 3, 0, 200], [20000, 1500, 700, 0], 6, 2, 64, True),
     ([260, 40], [3000, 2500], 3, 1, 128, False),
     ([2200, 300], [2200, 100], 16, 16, 128, True),  # cut, with query blocks that see no key
+    ([1] * 700 + [3000] + [130] * 500, None, 4, 1, 64, True),  # over 1024 sequences, one of them long
     ([300] + [260] * 40, [300] + [0] * 40, 40, 40, 64, True),  # many items without keys behind some with
     ([300] + [260] * 40 + [129], [300] + [0] * 40 + [129], 24, 4, 128, False),
 ]
