@@ -18,9 +18,11 @@
 // Bound: HBM, every q / k / v element read once and written once.  A thread
 // handles 8 pairs (two 16-byte chunks) at a time; the loads of its first
 // units are issued before the angles are computed, which hides their latency.
-// Measured: 16384 rows of 32 / 8 heads of 128 into an E4M3 cache 74 us (5.0
+// Measured: 16384 rows of 32 / 8 heads of 128 into an E4M3 cache 71 us (5.2
 // TB/s; 102 us with integer divisions for the places of a unit and unpacked
 // arithmetic), 3120 rows of 24 / 24 heads 16.3 us (4.7 TB/s), 64 rows 2.9 us.
+// A warp per token: 3120 rows 14 us, but the prompt 74 at best; 128, 192, 384 or
+// 512 threads or 8 tokens a CTA: the prompt no faster.
 // The units whose loads a thread keeps in flight: 2 or 3 the same, 6 slower
 // (registers).
 //
@@ -75,6 +77,37 @@ struct RopeAxesParams {
 
 __device__ __forceinline__ long long load_index(const void* p, long long i, int is64) {
   return is64 ? static_cast<const long long*>(p)[i] : static_cast<long long>(static_cast<const int*>(p)[i]);
+}
+
+// Two E4M3 codes of -f / s with r the rounded reciprocal of s: the product
+// -f r moved by r times its residual, f - (f r) s, which is the rounded
+// quotient (Markstein's division), so that a value on a code's border falls as
+// the quotient does; taken negative, because the residual of a zero is +0 and
+// -0 + -0 keeps a zero's sign where -0 + 0 does not.  The product is cut at 512
+// first: from 448 on every code is the largest one, and the residual of an
+// infinity would be NaN; a NaN comes back through the residual.  Not for scales
+// whose reciprocal or residual leaves fp32's normal range.  One conversion
+// instead of the two of a bracketed reciprocal, 16384 x (32 + 2 x 8) heads of
+// 128 into E4M3 74 -> 71 us.
+__device__ __forceinline__ uint32_t rope_minus_codes2(float2 f, float s, float r) {
+  float2 t = __fmul2_rn(f, make_float2(-r, -r));
+  t = make_float2(fminf(fmaxf(t.x, -512.f), 512.f), fminf(fmaxf(t.y, -512.f), 512.f));
+  const float2 e = __ffma2_rn(t, make_float2(s, s), f);
+  t = __ffma2_rn(e, make_float2(-r, -r), t);
+  return e4m3x2_rn_sat(t.x, t.y);
+}
+
+// The codes of a unit whose scale is beyond rope_minus_codes2: one branch a unit (a
+// branch at each pair took 4 us more, a call 18).
+__device__ __forceinline__ uint4 rope_divided_codes(const float2 (&fa)[4], const float2 (&fb)[4], float s) {
+  uint32_t o[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 u = e < 2 ? fa[2 * e] : fb[2 * e - 4], v = e < 2 ? fa[2 * e + 1] : fb[2 * e - 3];
+    o[e] = e4m3x2_rn_sat(__fdiv_rn(u.x, s), __fdiv_rn(u.y, s)) |
+           (e4m3x2_rn_sat(__fdiv_rn(v.x, s), __fdiv_rn(v.y, s)) << 16);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // CACHE: 0 none, 1 bf16, 2 E4M3.
@@ -234,16 +267,19 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_axes(const RopeAxesParams
       *reinterpret_cast<uint4*>(dst + w.b) = pack8x2(fb);
     } else {
       const float s = c ? p.scale[1][p.scale_per_head[1] ? w.head : 0] : p.scale[0][p.scale_per_head[0] ? w.head : 0];
-      const float r = QuantFp8::aux(s);
-      auto codes = [&](const float2 (&f)[4]) {
-        uint32_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = QuantFp8::q2(f[e], s, r);
-        return make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
-      };
+      uint4 o;
+      if (__builtin_expect(s > 0x1p-80f && s < 0x1p80f, 1)) {
+        const float r = __frcp_rn(s);
+        o.x = (rope_minus_codes2(fa[0], s, r) | (rope_minus_codes2(fa[1], s, r) << 16)) ^ 0x80808080u;
+        o.y = (rope_minus_codes2(fa[2], s, r) | (rope_minus_codes2(fa[3], s, r) << 16)) ^ 0x80808080u;
+        o.z = (rope_minus_codes2(fb[0], s, r) | (rope_minus_codes2(fb[1], s, r) << 16)) ^ 0x80808080u;
+        o.w = (rope_minus_codes2(fb[2], s, r) | (rope_minus_codes2(fb[3], s, r) << 16)) ^ 0x80808080u;
+      } else {
+        o = rope_divided_codes(fa, fb, s);
+      }
       uint8_t* dst = static_cast<uint8_t*>(cache) + at;
-      *reinterpret_cast<uint2*>(dst + w.a) = codes(fa);
-      *reinterpret_cast<uint2*>(dst + w.b) = codes(fb);
+      *reinterpret_cast<uint2*>(dst + w.a) = make_uint2(o.x, o.y);
+      *reinterpret_cast<uint2*>(dst + w.b) = make_uint2(o.z, o.w);
     }
   };
 #pragma unroll

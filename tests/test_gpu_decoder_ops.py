@@ -243,6 +243,25 @@ def test_rope_axes_store(kind, M, hq, hk, D, page, layout):
         assert (c[r // page, r % page] == 3).all()  # every other slot as it was
 
 
+def test_rope_axes_store_codes_of_every_value():
+    """E4M3 codes are the rounded fp32 quotient's for every bf16 value, zeros' signs, infinities and NaN included, and
+    for scales from fp32's least to its largest magnitudes (one per key head)."""
+    scales = torch.tensor([1e-41, 1e-38, 3e-25, 1e-12, 0.0137, 0.3, 1.0, 3.0, 448.0, 7e23, 3e24, 3e38], device=DEV)
+    hk, D = scales.numel(), 128
+    every = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(BF).to(DEV).view(512, 1, D)
+    v = every.expand(512, hk, D).reshape(512, hk * D).contiguous()
+    kc, vc = (torch.zeros(16, 32, hk, D, dtype=torch.uint8, device=DEV) for _ in range(2))
+    freqs, axes = K.rope_axes_frequencies((D // 2,), shared=True, device=DEV)
+    K.rope_axes_store(torch.zeros(512, D, dtype=BF, device=DEV), torch.zeros_like(v), v, torch.zeros(512, dtype=torch.int32, device=DEV),
+                      freqs, axes, D, kc, vc, torch.arange(512, device=DEV), interleaved=False, k_scale=scales, v_scale=scales)
+    quotient = v.float().view(512, hk, D) / scales[:, None]
+    want = quotient.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+    got, nan = vc.view(512, hk, D), quotient.isnan()
+    assert torch.equal(got[~nan], want[~nan])
+    assert ((got[nan] & 0x7f) == 0x7f).all()
+    assert (kc == 0).all()
+
+
 def test_rope_axes_store_index_and_code_types():
     """int32 slots and a float8_e4m3fn cache give what int64 slots and a uint8 cache give."""
     g = gen(2)
