@@ -49,7 +49,11 @@
 // are replaced (not added to), the V rows of the last 16-key step behind the
 // end are zeroed in shared memory, further steps are not multiplied, and
 // output rows are stored one by one.  So nothing, NaN included, passes from
-// one sequence to another.
+// one sequence to another.  Later keys of a query's own sequence take part in
+// its last step with probability zero, which times an infinity or a NaN is a
+// NaN: a row whose sum is finite and whose output is not is looked at again
+// (packed_mend), so that what a row does not see does not reach it either (the
+// look at the outputs takes 0.2 us of a short item's 4).
 #pragma once
 
 #include <cuda.h>
@@ -78,6 +82,8 @@ struct PackedParams {
   long long ldo;
   float* lse;        // [total_q, heads] or nullptr
   float* ws;         // partial results and records, or nullptr: items are never cut
+  const __nv_bfloat16 *q, *k, *v;  // as in the tensor maps, for packed_mend
+  long long ldq, ldk, ldv;
 };
 
 // Shared-memory descriptors as two words.  The high word is a constant (8-row
@@ -220,7 +226,96 @@ __host__ __device__ constexpr int packed_part_floats() { return 2 * 128 * (D + 2
 struct PackedRecord {
   int used, ends;           // there is a partial result; it is the item's last
   int row[2], rows[2], head[2];
+  int k0, end[2], limit[2];  // the item's first key row; keys in its steps; last visible key of the first row
 };
+
+// The rows of a warp (a lane each) once more whose sum is finite and whose
+// output holds a NaN (`bad`), where a key behind the row's last visible one
+// (`limit`) and inside the steps that were multiplied (`end`) has a value that
+// is not finite: 8 lanes to a key, 4 keys at a time, from global memory.  k and
+// v point at the sequence's first key, q_row and out_row at the lane's row, m
+// and inv are its maximum and 1 / sum.  `only` >= 0: just that eighth of the
+// columns is written.
+template <int D>
+__device__ __noinline__ void packed_mend(bool bad, int limit, int end, const __nv_bfloat16* q_row,
+                                         const __nv_bfloat16* k, long long ldk, const __nv_bfloat16* v, long long ldv,
+                                         __nv_bfloat16* out_row, float scale_log2e, float m, float inv, int only) {
+  constexpr int E = D / 8;
+  const int lane = threadIdx.x & 31, part = lane & 7, group = lane >> 3;
+  __syncwarp();  // the rows' first results are stored
+  int worst = -1;
+  for (int j = __reduce_min_sync(0xffffffffu, bad ? limit + 1 : end) + lane; j < end; j += 32) {
+    const uint4* at = reinterpret_cast<const uint4*>(v + j * ldv);
+    uint32_t most = 0;  // largest exponent field
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      const uint4 w = at[c];
+      most = __vmaxu2(most, __vmaxu2(__vmaxu2(w.x & 0x7f807f80u, w.y & 0x7f807f80u),
+                                     __vmaxu2(w.z & 0x7f807f80u, w.w & 0x7f807f80u)));
+    }
+    if ((most & 0xffffu) == 0x7f80u || (most >> 16) == 0x7f80u) worst = j;
+  }
+  worst = __reduce_max_sync(0xffffffffu, worst);
+  unsigned todo = __ballot_sync(0xffffffffu, bad && limit < worst);
+  auto row_of = [](unsigned long long ptr, int src) { return __shfl_sync(0xffffffffu, ptr, src); };
+  auto widen = [](const __nv_bfloat16* src, float (&f)[E]) {
+#pragma unroll
+    for (int c = 0; c < E / 8; ++c) {
+      const uint4 w4 = reinterpret_cast<const uint4*>(src)[c];
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[8 * c + 2 * i] = __uint_as_float(w[i] << 16);
+        f[8 * c + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  };
+  while (todo) {
+    const int src = __ffs(todo) - 1;
+    todo &= todo - 1;
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(row_of(reinterpret_cast<uintptr_t>(q_row), src));
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(row_of(reinterpret_cast<uintptr_t>(out_row), src));
+    const int n = __shfl_sync(0xffffffffu, limit, src) + 1;
+    const float row_m = __shfl_sync(0xffffffffu, m, src), row_inv = __shfl_sync(0xffffffffu, inv, src);
+    float qf[E], acc[E];
+    widen(q + part * E, qf);
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[i] = 0.f;
+#pragma unroll 1
+    for (int j0 = 0; j0 < n; j0 += 4) {
+      const int j = min(j0 + group, n - 1);
+      float kf[E], vf[E];
+      widen(k + j * ldk + part * E, kf);
+      widen(v + j * ldv + part * E, vf);
+      float dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) dot = fmaf(qf[i], kf[i], dot);
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      const float w = __bfloat162float(__float2bfloat16(ex2_approx(fmaf(dot, scale_log2e, -row_m))));
+      if (j0 + group < n) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[i] = fmaf(w, vf[i], acc[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 8);
+      acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 16);
+      acc[i] *= row_inv;
+    }
+    if (group == 0 && (only < 0 || only == part)) {
+#pragma unroll
+      for (int c = 0; c < E / 8; ++c) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = acc[8 * c + i];
+        reinterpret_cast<uint4*>(out + part * E)[c] = pack8(f);
+      }
+    }
+  }
+  __syncwarp();
+}
 
 // What an item costs beside its steps, in steps (measured: 4 us for an item of
 // one step, 1.8 us for every further one).
@@ -344,7 +439,10 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
                     r.row[t] = it.q0 + it.m[t];
                     r.rows[t] = max(0, min(128, it.lq - it.m[t]));
                     r.head[t] = it.head[t];
+                    r.end[t] = min(s.lk, 128 * packed_tile_steps(p, s, l0 + j, t));
+                    r.limit[t] = it.m[t] + it.diag + 128 * (n - to);
                   }
+                  r.k0 = s.k0;
                   rec[part] = r;
                 }
                 if (!put(it)) return;
@@ -772,12 +870,14 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         continue;
       }
       float inv = 0.f;  // a row that saw no key gives zeros
+      bool finite = false;
       if (steps > 0) {
         ok = mbar_wait_hot(&o_done[t], n_items++ & 1u, abort_flag, kTagPacked, 43);
         if (!ok) break;
         tc_fence_after();
         const float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
         if (m_use > -INFINITY) inv = 1.f / sum;
+        finite = m_use > -INFINITY && sum < INFINITY;
         if (lse != nullptr) *lse = m_use > -INFINITY ? (m_use + log2f(sum)) * 0.69314718055994531f : -INFINITY;
       } else if (lse != nullptr) {
         *lse = -INFINITY;
@@ -801,16 +901,22 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[c][i] = 0u;
       }
+      float2 nan2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};  // stays 0 but for infinities and NaN
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float f[8];
+            float2 f[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[2 * c + h][8 * i + e]) * inv;
-            *reinterpret_cast<uint4*>(box + lane * 128 + (((4 * h + i) ^ (lane & 7)) << 4)) = pack8(f);
+            for (int e = 0; e < 4; ++e)
+              f[e] = __fmul2_rn(make_float2(__uint_as_float(o[2 * c + h][8 * i + 2 * e]),
+                                            __uint_as_float(o[2 * c + h][8 * i + 2 * e + 1])),
+                                make_float2(inv, inv));
+            *reinterpret_cast<uint4*>(box + lane * 128 + (((4 * h + i) ^ (lane & 7)) << 4)) = pack8x2(f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) nan2[e & 1] = __ffma2_rn(f[e], make_float2(0.f, 0.f), nan2[e & 1]);
           }
         __syncwarp();
         __nv_bfloat16* to = lane_dst + 64 * c;
@@ -828,6 +934,14 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         __syncwarp();
       }
       tc_fence_before();
+      const int end = min(it->lk, 128 * steps);
+      const bool bad = finite && lane < rows && limit + 1 < end &&
+                       !((nan2[0].x + nan2[0].y) + (nan2[1].x + nan2[1].y) == 0.f);
+      if (__any_sync(0xffffffffu, bad)) {
+        const int col = head / p.group * D;
+        packed_mend<D>(bad, limit, end, p.q + (first + lane) * p.ldq + head * D, p.k + it->k0 * p.ldk + col, p.ldk,
+                       p.v + it->k0 * p.ldv + col, p.ldv, dst + lane * p.ldo, p.scale_log2e, m_use, inv, -1);
+      }
       release_item();
     }
   }
@@ -875,20 +989,31 @@ __global__ void __launch_bounds__(256) k_attn_packed_join(const PackedParams p, 
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = fmaf(w[(2 + warp * N + i) * 128], f, acc[i]);
   }
-  if (!live) return;
   const float inv = m > -INFINITY ? 1.f / sum : 0.f;
   const long long grow = (t ? r.row[1] : r.row[0]) + row;
   const int head = t ? r.head[1] : r.head[0];
-  __nv_bfloat16* dst = p.out + grow * p.ldo + head * D + warp * N;
+  __nv_bfloat16* dst = p.out + grow * p.ldo + head * D;
+  float nan = 0.f;  // stays 0 but for infinities and NaN
 #pragma unroll
-  for (int i = 0; i < N / 8; ++i) {
-    float f[8];
+  for (int i = 0; i < N; ++i) nan = fmaf(acc[i], 0.f, nan);
+  if (live) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = acc[8 * i + e] * inv;
-    reinterpret_cast<uint4*>(dst)[i] = pack8(f);
+    for (int i = 0; i < N / 8; ++i) {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = acc[8 * i + e] * inv;
+      reinterpret_cast<uint4*>(dst + warp * N)[i] = pack8(f);
+    }
+    if (p.lse != nullptr && warp == 0)
+      p.lse[grow * p.heads + head] = m > -INFINITY ? (m + log2f(sum)) * 0.69314718055994531f : -INFINITY;
   }
-  if (p.lse != nullptr && warp == 0)
-    p.lse[grow * p.heads + head] = m > -INFINITY ? (m + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+  const int end = t ? r.end[1] : r.end[0], limit = min(end - 1, (t ? r.limit[1] : r.limit[0]) + row);
+  const bool bad = live && m > -INFINITY && sum < INFINITY && limit + 1 < end && !(nan == 0.f);
+  if (__any_sync(0xffffffffu, bad)) {
+    const int col = head / p.group * D;
+    packed_mend<D>(bad, limit, end, p.q + grow * p.ldq + head * D, p.k + r.k0 * p.ldk + col, p.ldk,
+                   p.v + r.k0 * p.ldv + col, p.ldv, dst, p.scale_log2e, m, inv, warp);
+  }
 }
 
 }  // namespace qib

@@ -4,6 +4,8 @@
 // that module's device status word).
 #pragma once
 
+#include <cfloat>
+
 #include "attn_packed.cuh"
 #include "attn_paged.cuh"
 #include "rms_quant.cuh"
@@ -265,9 +267,10 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
   if (head_dim != 64 && head_dim != 128) return QI_B200_ESHAPE;
   if (n_seq < 0 || total_q < 0 || total_k < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return QI_B200_ESHAPE;
   if (n_seq == 0 || total_q == 0) return QI_B200_OK;
+  if (static_cast<long long>(total_q) + total_k > 0x3fffffff) return QI_B200_ETOOBIG;  // key places in 32 bits
   if (q == nullptr || out == nullptr || cu_q == nullptr || cu_k == nullptr || (total_k > 0 && (!k || !v)))
     return QI_B200_EINVAL;
-  if (!(scale > 0.0f)) return QI_B200_EINVAL;
+  if (!(scale > 0.0f) || scale > FLT_MAX) return QI_B200_EINVAL;
   const long long wq = static_cast<long long>(heads) * head_dim, wk = static_cast<long long>(kv_heads) * head_dim;
   if (ldq < wq || ldo < wq || ldq % 8 || ldo % 8) return QI_B200_ESHAPE;
   if (total_k > 0 && (ldk < wk || ldv < wk || ldk % 8 || ldv % 8)) return QI_B200_ESHAPE;
@@ -292,6 +295,12 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
   p.out = static_cast<__nv_bfloat16*>(out);
   p.ldo = ldo;
   p.lse = lse;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.ldq = ldq;
+  p.ldk = ldk;
+  p.ldv = ldv;
   return head_dim == 128 ? launch_packed<128>(q, ldq, k, ldk, v, ldv, p, di->num_sms, stream)
                          : launch_packed<64>(q, ldq, k, ldk, v, ldv, p, di->num_sms, stream);
 }
@@ -330,7 +339,7 @@ int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_ca
   if (q == nullptr || out == nullptr || lengths == nullptr || cache == nullptr || (max_pages > 0 && !page_table) ||
       workspace == nullptr)
     return QI_B200_EINVAL;
-  if (!(scale > 0.0f)) return QI_B200_EINVAL;
+  if (!(scale > 0.0f) || scale > FLT_MAX) return QI_B200_EINVAL;
   const long long wq = static_cast<long long>(heads) * head_dim;
   if (ldq < wq || ldo < wq || ldq % 8 || ldo % 8) return QI_B200_ESHAPE;
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace)) return QI_B200_EALIGN;

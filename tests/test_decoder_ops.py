@@ -185,7 +185,8 @@ def test_c_abi_refuses_before_it_touches_the_device():
     assert packed_(n=0) == packed_(tq=0) == _lib.OK
     assert packed_(D=96) == packed_(heads=3, kv=2) == packed_(ldq=128) == packed_(ldq=260) == _lib.ESHAPE
     assert packed_(q=None) == packed_(k=None) == packed_(cu=None) == packed_(scale=0.0) == _lib.EINVAL
-    assert packed_(scale=float("nan")) == _lib.EINVAL
+    assert packed_(scale=float("nan")) == packed_(scale=float("inf")) == _lib.EINVAL
+    assert packed_(tq=0x3fffffff) == _lib.ETOOBIG
     assert packed_(k=p + 8) == packed_(ws=p + 8) == _lib.EALIGN
     size = ref(ctypes.c_size_t())
     assert lib.qi_b200_attention_packed_workspace_bytes(1, 4, 4, 3, 2, 128, size) == _lib.ESHAPE
@@ -197,7 +198,7 @@ def test_c_abi_refuses_before_it_touches_the_device():
         lib.qi_b200_attention_paged(q, 256, ref(c), p, ld, mp, p, p, 256, None, B, heads, kv, D, scale, ws, nb, None)
     assert paged_(B=0) == _lib.OK
     assert paged_(D=32) == paged_(B=65536) == paged_(heads=3, kv=2) == paged_(ld=3) == _lib.ESHAPE
-    assert paged_(q=None) == paged_(ws=None) == paged_(scale=-1.0) == _lib.EINVAL
+    assert paged_(q=None) == paged_(ws=None) == paged_(scale=-1.0) == paged_(scale=float("inf")) == _lib.EINVAL
     assert paged_(q=p + 8) == paged_(ws=p + 8) == _lib.EALIGN
     assert paged_(mp=1 << 28, ld=1 << 28) == _lib.ETOOBIG  # lengths of 2^32 tokens
     assert paged_() == _lib.ECUDA

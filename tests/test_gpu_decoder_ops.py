@@ -426,6 +426,45 @@ def test_attention_packed_strided_and_rows_left_alone():
     assert torch.equal(p[:150], big[:150, 8:8 + hq * D]) and torch.isnan(p[150:T]).all()
 
 
+@pytest.mark.parametrize("ql,kl,hq,hk,D", [
+    ([300, 40], None, 2, 1, 128),        # pairs of heads
+    ([300, 40], None, 3, 3, 64),         # one head, two query tiles
+    ([129], [9000], 2, 2, 128),          # cut over the SMs and joined
+    ([130, 77], [6000, 5100], 4, 2, 64),
+])
+def test_attention_packed_later_keys_do_not_reach_a_query(ql, kl, hq, hk, D):
+    """Infinities and NaN in keys and values that causality hides: a query in front of them is as without them, one
+    behind them has them in their columns (a value) or in all (a key)."""
+    kl = kl or ql
+    g = gen(sum(kl) + D)
+    q, k, v = randn(g, sum(ql), hq * D), randn(g, sum(kl), hk * D), randn(g, sum(kl), hk * D)
+    lq, lk = ql[0], kl[0]
+    bad_v, bad_k, columns = lk - 70, lk - 25, (5, D - 3)  # keys of the first sequence
+    zeroed = v.clone()
+    zeroed[bad_v, list(columns)] = 0
+    want, tol, wl = packed_ref(q, k, zeroed, ql, kl, hq, hk, D, True, D ** -0.5)
+    v[bad_v, columns[0]], v[bad_v, columns[1]] = float("nan"), float("inf")
+    clean = k.clone()
+    k[bad_k] = float("nan")
+    lse = torch.empty(sum(ql), hq, device=DEV)
+    o = K.attention_packed(q, k, v, cu(ql), cu(kl), hq, hk, lse=lse)
+    after_v, after_k = bad_v - (lk - lq), bad_k - (lk - lq)  # the first queries that see them
+    hit = torch.zeros(sum(ql), hq, D, dtype=torch.bool, device=DEV)
+    for h in range(hq // hk):  # the value's columns belong to key head 0
+        hit[after_v:lq, h, list(columns)] = True
+    hit[after_k:lq] = True
+    hit = hit.view(sum(ql), hq * D)
+    assert not torch.isfinite(o[hit]).any() and torch.isnan(o[after_k:lq]).all()
+    assert ((o.double() - want).abs() <= tol)[~hit].all()
+    close_lse(torch.cat([lse[:after_k], lse[lq:]]), torch.cat([wl[:after_k], wl[lq:]]))
+    # the same without the key: only the value's columns are lost
+    o = K.attention_packed(q, clean, v, cu(ql), cu(kl), hq, hk)
+    hit = hit.view(sum(ql), hq, D)
+    hit[after_k:lq] = hit[after_v]
+    hit = hit.view(sum(ql), hq * D)
+    assert not torch.isfinite(o[hit]).any() and ((o.double() - want).abs() <= tol)[~hit].all()
+
+
 def test_attention_packed_nothing_to_do():
     q = torch.zeros(0, 128, dtype=BF, device=DEV)
     assert K.attention_packed(q, q, q, cu([]), cu([]), 1, 1).shape == (0, 128)
