@@ -876,9 +876,10 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         if (!ok) break;
         tc_fence_after();
         const float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-        if (m_use > -INFINITY) inv = 1.f / sum;
-        finite = m_use > -INFINITY && sum < INFINITY;
-        if (lse != nullptr) *lse = m_use > -INFINITY ? (m_use + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+        // a sum of NaN (with a maximum that is still -inf where every score is one) stays one
+        if (sum != 0.f) inv = 1.f / sum;
+        finite = sum > 0.f && sum < INFINITY;
+        if (lse != nullptr) *lse = sum != 0.f ? (m_use + log2f(sum)) * 0.69314718055994531f : -INFINITY;
       } else if (lse != nullptr) {
         *lse = -INFINITY;
       }
@@ -983,13 +984,13 @@ __global__ void __launch_bounds__(256) k_attn_packed_join(const PackedParams p, 
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
   for (int c = c0; c <= c1; ++c) {
     const float* w = part(c);
-    if (w[0] == -INFINITY) continue;  // saw no key: nothing was written behind the sum
+    if (w[128] == 0.f) continue;  // saw no key: nothing was written behind the sum
     const float f = ex2_approx(w[0] - m);
     sum = fmaf(w[128], f, sum);
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = fmaf(w[(2 + warp * N + i) * 128], f, acc[i]);
   }
-  const float inv = m > -INFINITY ? 1.f / sum : 0.f;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
   const long long grow = (t ? r.row[1] : r.row[0]) + row;
   const int head = t ? r.head[1] : r.head[0];
   __nv_bfloat16* dst = p.out + grow * p.ldo + head * D;
@@ -1005,10 +1006,10 @@ __global__ void __launch_bounds__(256) k_attn_packed_join(const PackedParams p, 
       reinterpret_cast<uint4*>(dst + warp * N)[i] = pack8(f);
     }
     if (p.lse != nullptr && warp == 0)
-      p.lse[grow * p.heads + head] = m > -INFINITY ? (m + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+      p.lse[grow * p.heads + head] = sum != 0.f ? (m + log2f(sum)) * 0.69314718055994531f : -INFINITY;
   }
   const int end = t ? r.end[1] : r.end[0], limit = min(end - 1, (t ? r.limit[1] : r.limit[0]) + row);
-  const bool bad = live && m > -INFINITY && sum < INFINITY && limit + 1 < end && !(nan == 0.f);
+  const bool bad = live && sum > 0.f && sum < INFINITY && limit + 1 < end && !(nan == 0.f);
   if (__any_sync(0xffffffffu, bad)) {
     const int col = head / p.group * D;
     packed_mend<D>(bad, limit, end, p.q + grow * p.ldq + head * D, p.k + r.k0 * p.ldk + col, p.ldk,

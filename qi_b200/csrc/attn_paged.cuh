@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
         acc.y = fmaf(v.y, f, acc.y);
       }
       if (whole) {
-        const float inv = l > 0.f ? v_scale / l : 0.f;
+        const float inv = l != 0.f ? v_scale / l : 0.f;  // a sum of NaN stays one
         *reinterpret_cast<__nv_bfloat162*>(p.out + static_cast<long long>(b) * p.ldo + static_cast<long long>(head) * D +
                                            d) = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
         if (p.lse != nullptr && d == 0)
@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(kPagedJoinWarps * 32) k_attn_paged_join(const 
       o = fmaf(sm_o[w][d], f, o);
     }
     p.out[static_cast<long long>(r.b) * p.ldo + static_cast<long long>(head) * D + d] =
-        __float2bfloat16_rn(sum > 0.f ? o / sum : 0.f);
+        __float2bfloat16_rn(sum != 0.f ? o / sum : 0.f);
     if (p.lse != nullptr && d == 0)
       p.lse[static_cast<long long>(r.b) * p.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
   }

@@ -465,6 +465,26 @@ def test_attention_packed_later_keys_do_not_reach_a_query(ql, kl, hq, hk, D):
     assert not torch.isfinite(o[hit]).any() and ((o.double() - want).abs() <= tol)[~hit].all()
 
 
+@pytest.mark.parametrize("ql,kl", [([40, 300], [40, 300]), ([129], [9000])])
+def test_attention_packed_nan_queries_and_keys(ql, kl):
+    """A NaN in a query is in its row's output and lse, a NaN in a key in those of every query that sees it, whole
+    items and cut ones alike; no other row changes."""
+    g = gen(sum(kl))
+    hq, hk, D = 2, 1, 128
+    q, k, v = randn(g, sum(ql), hq * D), randn(g, sum(kl), hk * D), randn(g, sum(kl), hk * D)
+    lse, lse0 = (torch.empty(sum(ql), hq, device=DEV) for _ in range(2))
+    plain = K.attention_packed(q, k, v, cu(ql), cu(kl), hq, hk, lse=lse0)
+    q[20, 3] = float("nan")  # head 0
+    k[kl[0] - 10, 7] = float("nan")
+    o = K.attention_packed(q, k, v, cu(ql), cu(kl), hq, hk, lse=lse)
+    hit = torch.zeros(sum(ql), hq, dtype=torch.bool, device=DEV)
+    hit[20, 0] = True
+    hit[ql[0] - 10:ql[0]] = True
+    o, plain = o.view(-1, hq, D), plain.view(-1, hq, D)
+    assert torch.isnan(o[hit]).all() and torch.isnan(lse[hit]).all()
+    assert torch.equal(o[~hit], plain[~hit]) and torch.equal(lse[~hit], lse0[~hit])
+
+
 def test_attention_packed_nothing_to_do():
     q = torch.zeros(0, 128, dtype=BF, device=DEV)
     assert K.attention_packed(q, q, q, cu([]), cu([]), 1, 1).shape == (0, 128)
@@ -575,6 +595,39 @@ def test_attention_paged_garbage_behind_the_length(kind):
         kc[last, (m - 1) % 16 + 1:] = nan
         vc[last, (m - 1) % 16 + 1:] = nan
     assert torch.equal(o, K.attention_paged(q, kc, vc, table, n, k_scale=ks, v_scale=vs))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("lens", [[40] * 300, [5000, 33]])
+def test_attention_paged_nan_queries_and_keys(kind, lens):
+    """A NaN in a query head is in that head's output and lse, a NaN in a cached key in those of its sequence's heads,
+    items inside one range and items cut by ranges alike; no other row changes."""
+    g = gen(sum(lens))
+    hq, hk, D, page = 4, 2, 128, 16
+    q = randn(g, len(lens), hq * D)
+    n = [-(-m // page) for m in lens]
+    kc, vc = (randn(g, sum(n) * page * hk, D).view(sum(n), page, hk, D) for _ in range(2))
+    kw = {}
+    if kind == "fp8":
+        kc, vc = (c.to(torch.float8_e4m3fn) for c in (kc, vc))
+        kw = {"k_scale": torch.ones(1, device=DEV), "v_scale": torch.ones(1, device=DEV)}
+    pages = torch.zeros(len(lens), max(n), dtype=torch.int32)
+    at = 0
+    for i, c in enumerate(n):
+        pages[i, :c] = torch.arange(at, at + c)
+        at += c
+    pages, lengths = pages.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    lse, lse0 = (torch.empty(len(lens), hq, device=DEV) for _ in range(2))
+    plain = K.attention_paged(q, kc, vc, pages, lengths, lse=lse0, **kw)
+    q[0, 2 * D + 5] = float("nan")  # sequence 0, head 2
+    kc[n[0], 3, 1, 9] = float("nan")  # sequence 1, key head 1: heads 2 and 3
+    o = K.attention_paged(q, kc, vc, pages, lengths, lse=lse, **kw)
+    hit = torch.zeros(len(lens), hq, dtype=torch.bool, device=DEV)
+    hit[0, 2] = True
+    hit[1, 2:] = True
+    o, plain = o.view(-1, hq, D), plain.view(-1, hq, D)
+    assert torch.isnan(o[hit]).all() and torch.isnan(lse[hit]).all()
+    assert torch.equal(o[~hit], plain[~hit]) and torch.equal(lse[~hit], lse0[~hit])
 
 
 def test_attention_paged_bad_pages_and_lengths_are_left_out():
