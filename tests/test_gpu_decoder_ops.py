@@ -710,6 +710,53 @@ def test_side_stream_and_graph_replay():
     assert all(torch.equal(a, b) for a, b in zip(got, want[3]))
 
 
+def test_offsets_beyond_32_bits():
+    """Rows and cache pages more than 2^32 elements behind the first give what the same values give close together."""
+    g = gen(77)
+    free = torch.cuda.mem_get_info()[0]
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    M, hq, hk, D = 4200, 2, 1, 128
+    wide = torch.empty(M, 1 << 20, dtype=BF, device=DEV)  # 8.8 GB
+    near = {n: randn(g, M, h * D) for n, h in (("q", hq), ("k", hk), ("v", hk), ("y", hq))}
+    far, at = {}, 8
+    for n, x in near.items():
+        far[n] = wide[:, at:at + x.size(1)]
+        far[n].copy_(x)
+        at += x.size(1)
+    w = randn(g, 1, hq * D)[0]
+    out = wide[:, 1 << 19:(1 << 19) + hq * D]
+    codes, scales = K.rms_norm_quant(_lib.KIND_FP8_E4M3, far["q"], w, far["y"], x_out=out)
+    stream = near["q"].clone()
+    want = K.rms_norm_quant(_lib.KIND_FP8_E4M3, stream, w, near["y"])
+    assert torch.equal(codes, want[0]) and torch.equal(scales, want[1]) and torch.equal(out, stream)
+    freqs, axes = K.rope_axes_frequencies((D // 2,), shared=True, device=DEV)
+    pos = torch.arange(M, dtype=torch.int32, device=DEV)
+    want = K.rope_axes(near["q"], near["k"], pos, freqs, axes, D)
+    K.rope_axes(far["q"], far["k"], pos, freqs, axes, D, out_q=far["q"], out_k=far["k"])
+    assert torch.equal(far["q"], want[0]) and torch.equal(far["k"], want[1])
+    n = cu([M - 300, 300])
+    K.attention_packed(far["q"], far["k"], far["v"], n, n, hq, hk, out=out)
+    assert torch.equal(out, K.attention_packed(*want, near["v"], n, n, hq, hk))
+    del wide, far, out
+    # 100 tokens in the last pages of a cache, against the same pages alone
+    pages, page, hk = (1 << 16) + 3, 64, 8
+    cache = torch.empty(pages, 2, page, hk, D, dtype=torch.uint8, device=DEV)  # 8.6 GB
+    few = torch.zeros(3, 2, page, hk, D, dtype=torch.uint8, device=DEV)
+    cache[-3:] = 0
+    k, v, q = randn(g, 100, hk * D), randn(g, 100, hk * D), randn(g, 100, hk * D)
+    s = torch.ones(1, device=DEV)
+    slots = torch.randperm(3 * page, generator=g)[:100].to(DEV)
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([3 * page], dtype=torch.int32, device=DEV)
+    got = []
+    for c, first in ((cache, pages - 3), (few, 0)):
+        K.rope_axes_store(q, k, v, pos[:100], freqs, axes, D, c[:, 0], c[:, 1], slots + first * page, k_scale=s, v_scale=s)
+        got.append(K.attention_paged(q[:1], c[:, 0], c[:, 1], table + first, lengths, k_scale=s, v_scale=s))
+    assert torch.equal(cache[-3:], few) and torch.equal(got[0], got[1])
+    _lib.raise_on_device_error()
+
+
 def test_refusals():
     x = torch.zeros(4, 256, dtype=BF, device=DEV)
     w = torch.ones(256, dtype=BF, device=DEV)
