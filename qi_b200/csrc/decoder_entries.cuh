@@ -250,7 +250,7 @@ int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk
   }
   // tokens per CTA: one where there are few (64 rows 2.9 us against 3.4 with two),
   // two from four CTAs per SM up (3120 rows 16.3 us against 18.4 and 17.1 with one
-  // and four), four from eight up (16384 rows 74 us against 80 with two)
+  // and four), four from eight up (16384 rows 70 us against 77 with two)
   p.tokens = M >= 4 * 8 * di->num_sms ? kRopeMaxTokens : (M >= 2 * 4 * di->num_sms ? 2 : 1);
   const long long units = static_cast<long long>(heads + (cache ? 2 : 1) * kv_heads) * (head_dim / 16);
   if (ldq > kRopeMaxStride || ldk > kRopeMaxStride || ldv > kRopeMaxStride || units > kRopeMaxUnits)

@@ -9,7 +9,13 @@
 //
 // Mathematics: with r = 1 / sqrt(mean(h^2) + eps), v = (h w) r and
 // max|v| = r max|h w|, so sum(h^2) and max|h w| come out of ONE reduction over
-// the row, and the code of an element is one product, (h w) (r / s).
+// the row.  Where s is not its floor, r cancels from v / s: the quotient is
+// (h w) k with k = 127 / max|h w| (448 for E4M3); h w and the maximum are exact
+// in fp32 (16 bits).  k is held as k_hi + k_lo, and the code is that of
+// fma(h w, k_hi, (h w) k_lo), the quotient rounded once: codes fall as those of
+// exact arithmetic do, ties included (the product (h w) (r / s) tipped one in
+// 10^5, for one packed operation per two elements less: 144 us against 146 for
+// 16384 x 8192 with residual).
 //
 // Bound: HBM, 2 D in (+ 2 D of y), D codes out (+ 2 D of h) per row.
 // A row lives in the registers of T threads (16-byte chunks, C per thread)
@@ -23,6 +29,7 @@
 #include "dit_fused.cuh"
 #include "launch_count.cuh"
 #include "quantize_act.cuh"
+#include "quantize_nvfp4.cuh"
 
 namespace qib {
 
@@ -128,7 +135,17 @@ __global__ void __launch_bounds__(512) k_rms_quant(const RmsQuantParams p, int T
   float s = 1.f;
   if (FMT == 1) s = amax == amax ? fmaxf(__fdiv_rn(amax, 127.0f), 1e-10f) : amax;
   if (FMT == 2) s = amax == amax ? fmaxf(__fdiv_rn(amax, 448.0f), 1e-12f) : amax;
-  const float k = __fdiv_rn(r, s);
+  // v / s = (h w) (k_hi + k_lo).  k_hi lies below k by 2^-22 to 2^-20 of it, more
+  // than the reciprocal's error, so k_lo is positive and a zero keeps its sign; the
+  // residual is exact (20 bits), and the sum is right to 2^-40 of k
+  constexpr float kTop = FMT == 1 ? 127.f : 448.f, kFloor = FMT == 1 ? 1e-10f : 1e-12f;
+  const float inv = rcp_approx(mx);
+  float k_hi = inv * (kTop - kTop * 0x1p-21f);
+  float k_lo = fmaf(-k_hi, mx, kTop) * inv;
+  if (!(amax >= kFloor * kTop && mx > 0x1p-80f && mx < 0x1p80f)) {  // s is its floor, or the row has none
+    k_hi = __fdiv_rn(r, s);
+    k_lo = 0.f;
+  }
   if (FMT != 0 && live && t == 0) p.s[row] = s;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -140,10 +157,10 @@ __global__ void __launch_bounds__(512) k_rms_quant(const RmsQuantParams p, int T
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = __fmul2_rn(f[e], w[e]);
     if (FMT != 0) {
-      const float2 k2 = make_float2(k, k);
       float2 v[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(f[e], k2);
+      for (int e = 0; e < 4; ++e)
+        v[e] = __ffma2_rn(f[e], make_float2(k_hi, k_hi), __fmul2_rn(f[e], make_float2(k_lo, k_lo)));
       reinterpret_cast<uint2*>(p.q + static_cast<long long>(row) * p.D)[j] =
           make_uint2(rms_codes4<FMT == 2>(v[0].x, v[0].y, v[1].x, v[1].y),
                      rms_codes4<FMT == 2>(v[2].x, v[2].y, v[3].x, v[3].y));

@@ -18,7 +18,7 @@
 // Bound: HBM, every q / k / v element read once and written once.  A thread
 // handles 8 pairs (two 16-byte chunks) at a time; the loads of its first
 // units are issued before the angles are computed, which hides their latency.
-// Measured: 16384 rows of 32 / 8 heads of 128 into an E4M3 cache 71 us (5.2
+// Measured: 16384 rows of 32 / 8 heads of 128 into an E4M3 cache 70 us (5.3
 // TB/s; 102 us with integer divisions for the places of a unit and unpacked
 // arithmetic), 3120 rows of 24 / 24 heads 16.3 us (4.7 TB/s), 64 rows 2.9 us.
 // A warp per token: 3120 rows 14 us, but the prompt 74 at best; 128, 192, 384 or
@@ -79,25 +79,18 @@ __device__ __forceinline__ long long load_index(const void* p, long long i, int 
   return is64 ? static_cast<const long long*>(p)[i] : static_cast<long long>(static_cast<const int*>(p)[i]);
 }
 
-// Two E4M3 codes of -f / s with r the rounded reciprocal of s: the product
-// -f r moved by r times its residual, f - (f r) s, which is the rounded
-// quotient (Markstein's division), so that a value on a code's border falls as
-// the quotient does; taken negative, because the residual of a zero is +0 and
-// -0 + -0 keeps a zero's sign where -0 + 0 does not.  The product is cut at 512
-// first: from 448 on every code is the largest one, and the residual of an
-// infinity would be NaN; a NaN comes back through the residual.  Not for scales
-// whose reciprocal or residual leaves fp32's normal range.  One conversion
-// instead of the two of a bracketed reciprocal, 16384 x (32 + 2 x 8) heads of
-// 128 into E4M3 74 -> 71 us.
-__device__ __forceinline__ uint32_t rope_minus_codes2(float2 f, float s, float r) {
-  float2 t = __fmul2_rn(f, make_float2(-r, -r));
-  t = make_float2(fminf(fmaxf(t.x, -512.f), 512.f), fminf(fmaxf(t.y, -512.f), 512.f));
-  const float2 e = __ffma2_rn(t, make_float2(s, s), f);
-  t = __ffma2_rn(e, make_float2(-r, -r), t);
-  return e4m3x2_rn_sat(t.x, t.y);
+// Two E4M3 codes of f / s, the reciprocal of s as a sum hi + lo: the quotient is
+// rounded once, so that a value on a code's border falls as the quotient does.
+// hi is rounded towards zero and lo positive: a zero keeps its sign, and an
+// infinity does not meet a zero.  Not for scales whose reciprocal or its
+// residual leaves fp32's normal range.  (Two codes from a bracketed reciprocal
+// took 74 us for the prompt above.)
+__device__ __forceinline__ uint32_t rope_codes2(float2 f, float hi, float lo) {
+  const float2 v = __ffma2_rn(f, make_float2(hi, hi), __fmul2_rn(f, make_float2(lo, lo)));
+  return e4m3x2_rn_sat(v.x, v.y);
 }
 
-// The codes of a unit whose scale is beyond rope_minus_codes2: one branch a unit (a
+// The codes of a unit whose scale is beyond rope_codes2: one branch a unit (a
 // branch at each pair took 4 us more, a call 18).
 __device__ __forceinline__ uint4 rope_divided_codes(const float2 (&fa)[4], const float2 (&fb)[4], float s) {
   uint32_t o[4];
@@ -269,11 +262,11 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_axes(const RopeAxesParams
       const float s = c ? p.scale[1][p.scale_per_head[1] ? w.head : 0] : p.scale[0][p.scale_per_head[0] ? w.head : 0];
       uint4 o;
       if (__builtin_expect(s > 0x1p-80f && s < 0x1p80f, 1)) {
-        const float r = __frcp_rn(s);
-        o.x = (rope_minus_codes2(fa[0], s, r) | (rope_minus_codes2(fa[1], s, r) << 16)) ^ 0x80808080u;
-        o.y = (rope_minus_codes2(fa[2], s, r) | (rope_minus_codes2(fa[3], s, r) << 16)) ^ 0x80808080u;
-        o.z = (rope_minus_codes2(fb[0], s, r) | (rope_minus_codes2(fb[1], s, r) << 16)) ^ 0x80808080u;
-        o.w = (rope_minus_codes2(fb[2], s, r) | (rope_minus_codes2(fb[3], s, r) << 16)) ^ 0x80808080u;
+        const float hi = __frcp_rz(s), lo = fmaxf(fmaf(-hi, s, 1.f), 0x1p-60f) * hi;
+        o.x = rope_codes2(fa[0], hi, lo) | (rope_codes2(fa[1], hi, lo) << 16);
+        o.y = rope_codes2(fa[2], hi, lo) | (rope_codes2(fa[3], hi, lo) << 16);
+        o.z = rope_codes2(fb[0], hi, lo) | (rope_codes2(fb[1], hi, lo) << 16);
+        o.w = rope_codes2(fb[2], hi, lo) | (rope_codes2(fb[3], hi, lo) << 16);
       } else {
         o = rope_divided_codes(fa, fb, s);
       }

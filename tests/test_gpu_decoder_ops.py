@@ -105,6 +105,30 @@ def test_rms_norm_quant(kind, M, D, residual):
         assert torch.equal(q, q2) and torch.equal(s, s2)
 
 
+@pytest.mark.parametrize("kind", [_lib.KIND_INT8, _lib.KIND_FP8_E4M3])
+@pytest.mark.parametrize("mul", [1e-9, 0.03, 1.0, 300.0])
+def test_rms_norm_quant_codes_are_those_of_exact_arithmetic(kind, mul):
+    """Where the scale is not its floor, v / s is top h w / max|h w| whatever the norm is, a quotient of values that
+    fp32 holds exactly, and its codes are those of the fp64 quotient.  Rounding it to fp32 first cannot move it onto a
+    code's border: with n, d < 2^16 the significands of h w and of the maximum, a quotient that is not on a border is
+    1 / (254 n) > 2^-24 of itself or more from one for INT8, 1 / (7 n) or 1 / (31 d) for E4M3."""
+    g = gen(int(mul * 1000) + kind)
+    M, D = 400, 2048
+    x, w = randn(g, M, D, mul=mul), randn(g, D)
+    q, s = K.rms_norm_quant(kind, x, w, eps=0.0)
+    t = (x.double() * w.double()).cpu()  # powers of two are exact there; the device's pow is not
+    top = 127.0 if kind == _lib.KIND_INT8 else 448.0
+    v = t * top / t.abs().amax(1, keepdim=True)
+    if kind == _lib.KIND_INT8:
+        assert torch.equal(q.cpu().double(), v.round())
+    else:
+        # fp64 -> E4M3 by hand: 8 steps to a binade, ties to even
+        step = 2.0 ** (torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -6))).clamp(-6, 8) - 3)
+        got = e4m3_value(q.cpu())
+        assert torch.equal(got, torch.round(v / step) * step)
+        assert torch.equal(torch.signbit(got), torch.signbit(v))
+
+
 def test_rms_norm_quant_strided_rows():
     g = gen(4)
     M, D = 50, 640
