@@ -315,8 +315,8 @@ int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk
  * out, fp32 scores and sums, probabilities rounded to bf16 before the product
  * with V.  lse (optional, fp32 [total_q, heads]): log of the sum of
  * exp(scale q.k), -inf where no key is seen.  Rows of out (and lse) outside
- * every sequence are left as they were.  Keys and values inside a sequence
- * have to be finite.  With a workspace of the size that
+ * every sequence are left as they were.  An infinity or a NaN reaches the
+ * queries that see it and no others.  out must not overlap the inputs.  With a workspace of the size that
  * qi_b200_attention_packed_workspace_bytes names (0: none is of use), items
  * may be cut over several SMs where they do not fill the device evenly; it
  * needs no initialization and may be used again by the next call on the
@@ -333,7 +333,8 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
  * pages are page_table[b, :] (int32, device, row stride ld_table, max_pages
  * columns).  A length of 0 gives zeros (lse -inf).  A page outside the cache
  * or a length behind the table reads nothing: those keys take no part, and
- * the device status word is set (code 2).  The workspace holds partial
+ * the device status word is set (code 2).  out must not overlap the inputs.
+ * The workspace holds partial
  * results of sequences that several SMs share; it needs no initialization and
  * may be used again by the next call on the stream. */
 int qi_b200_attention_paged_workspace_bytes(int kv_heads, int head_dim, size_t* bytes);

@@ -640,8 +640,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     (int32 [n + 1]).  ``causal``: query i sees the keys j <= i + (lk - lq), so
     the last query sees every key; a query that sees none gives zeros.  Query
     head h reads key head h // (heads // kv_heads).  Returns [Tq, heads * D]
-    bf16 (or writes ``out``; its rows outside every sequence stay as they
-    were).  ``lse`` fp32 [Tq, heads] receives the log of the softmax sums.
+    bf16 (or writes ``out``, which must not overlap the inputs; its rows
+    outside every sequence stay as they were).  ``lse`` fp32 [Tq, heads] receives the log of the softmax sums.
     Default scale 1 / sqrt(D)."""
     return _op("attention_packed", q, k, v, cu_q, cu_k, heads, kv_heads, causal, scale, out, lse)
 
@@ -660,5 +660,5 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     sequence's last page are not read; a page outside the cache, or a length
     behind the table, is left out and reported by
     ``_lib.raise_on_device_error``.  Returns [B, heads * D] bf16 (or writes
-    ``out``); ``lse`` fp32 [B, heads] receives the log of the softmax sums."""
+    ``out``, which must not overlap the inputs); ``lse`` fp32 [B, heads] receives the log of the softmax sums."""
     return _op("attention_paged", q, k_cache, v_cache, pages, lengths, scale, k_scale, v_scale, out, lse)
