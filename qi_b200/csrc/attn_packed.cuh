@@ -52,8 +52,9 @@
 // one sequence to another.  Later keys of a query's own sequence take part in
 // its last step with probability zero, which times an infinity or a NaN is a
 // NaN: a row whose sum is finite and whose output is not is looked at again
-// (packed_mend), so that what a row does not see does not reach it either (the
-// look at the outputs takes 0.2 us of a short item's 4).
+// (packed_mend), and one that saw no key at all is overwritten with zeros, so
+// that what a row does not see does not reach it either (the look at the outputs
+// takes 0.2 us of a short item's 4).
 #pragma once
 
 #include <cuda.h>
@@ -936,8 +937,16 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       }
       tc_fence_before();
       const int end = min(it->lk, 128 * steps);
-      const bool bad = finite && lane < rows && limit + 1 < end &&
-                       !((nan2[0].x + nan2[0].y) + (nan2[1].x + nan2[1].y) == 0.f);
+      const bool odd = lane < rows && !((nan2[0].x + nan2[0].y) + (nan2[1].x + nan2[1].y) == 0.f);
+      const bool bad = odd && finite && limit + 1 < end;
+      // a row that saw no key, in a tile whose step multiplied an infinity or a NaN
+      // (0 times which is a NaN): zeros
+      const bool blank = odd && inv == 0.f;
+      if (__any_sync(0xffffffffu, blank)) {
+        __syncwarp();  // the rows' first results are stored
+        if (blank)
+          for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(dst + lane * p.ldo)[c] = make_uint4(0u, 0u, 0u, 0u);
+      }
       if (__any_sync(0xffffffffu, bad)) {
         const int col = head / p.group * D;
         packed_mend<D>(bad, limit, end, p.q + (first + lane) * p.ldq + head * D, p.k + it->k0 * p.ldk + col, p.ldk,

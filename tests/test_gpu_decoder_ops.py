@@ -509,6 +509,36 @@ def test_attention_packed_nan_queries_and_keys(ql, kl):
     assert torch.equal(o[~hit], plain[~hit]) and torch.equal(lse[~hit], lse0[~hit])
 
 
+@pytest.mark.parametrize("ql,kl,hq,hk,D", [
+    ([300], [100], 2, 1, 128),           # pairs of heads: tokens 128 to 199 share a tile with some that see keys
+    ([300], [100], 1, 1, 64),            # one head, two query tiles
+    ([300, 70], [100, 0], 3, 3, 128),
+    ([1500, 2000], [1400, 1990], 4, 2, 128),  # the steps cut evenly over the SMs
+    ([1500, 2000], [1400, 1990], 3, 1, 64),
+])
+def test_attention_packed_queries_without_a_key_give_zeros(ql, kl, hq, hk, D):
+    """Queries in front of every key give zeros (lse -inf) whatever the keys and values hold; behind them, only those
+    that see an infinity or a NaN have it."""
+    g = gen(sum(ql) + hq + D)
+    q, k, v = randn(g, sum(ql), hq * D), randn(g, sum(kl), hk * D), randn(g, sum(kl), hk * D)
+    lq, lk = ql[0], kl[0]
+    want, tol, wl = packed_ref(q, k, v, ql, kl, hq, hk, D, True, D ** -0.5)
+    v[lk - 2], v[lk - 1], k[lk - 1, ::3] = float("nan"), float("inf"), float("nan")
+    lse = torch.empty(sum(ql), hq, device=DEV)
+    o = K.attention_packed(q, k, v, cu(ql), cu(kl), hq, hk, lse=lse)
+    first = 0
+    for a, b in zip(ql, kl):
+        none = slice(first, first + max(0, a - b))
+        assert (o[none] == 0).all() and (lse[none] == -math.inf).all()
+        first += a
+    hit = torch.zeros(sum(ql), dtype=torch.bool, device=DEV)
+    hit[lq - 2:lq] = True
+    assert torch.isnan(o[hit]).all()
+    assert ((o.double() - want).abs() <= tol)[~hit].all()
+    hit[lq - 2] = False  # it sees a value only
+    close_lse(lse[~hit], wl[~hit])
+
+
 def test_attention_packed_nothing_to_do():
     q = torch.zeros(0, 128, dtype=BF, device=DEV)
     assert K.attention_packed(q, q, q, cu([]), cu([]), 1, 1).shape == (0, 128)
