@@ -26,16 +26,20 @@
 // are the 8 columns of mma.sync m16n8k16: S^T = K Q^T (16 tokens x 8 heads) and
 // O^T += V^T P^T (16 columns x 8 heads); 9 to 16 heads take two column tiles
 // over the same K and V fragments.  P^T goes from S^T's accumulator layout to
-// the operand layout with one 8 x 8 transpose per 8 tokens.  The maximum in use
-// follows only when a row outgrew it by more than 2^8, so most blocks need one
-// vote and no reduction.  The tensor work is a few per cent of what the SM can
+// the operand layout with one 8 x 8 transpose per 8 tokens.  Powers P = 2^(s - base)
+// are taken above a base that follows the maximum; bf16 caches let it lag by
+// up to 2^8, so most blocks need one vote and no reduction.  The tensor work is a few per cent of what the SM can
 // do, so the legacy instruction is enough; what counts are the bytes in flight
 // (128 KB per SM) and the instructions per byte.
 //
 // E4M3 caches: codes are widened exactly to fp16 and multiplied in fp16 with
 // fp32 sums; q is scaled by a power of two per head so that it fits fp16, the
 // key scale goes into the softmax scale and the value scale into the output.
-// P is at most 2^8, inside fp16's range.
+// P is rounded to fp16, whose range ends at 2^-24: what lies far below a row's
+// maximum would be lost, although it makes up the output where the maximum's own
+// value is near zero.  So the base is 2^15 below the maximum and does not lag:
+// P reaches up to 2^15 and keeps its 11 bits down to 2^-29 of the maximum (20
+// nats), and no probability is off by more than 2^-40.
 //
 // A page index outside the cache, or a length behind the page table, reads
 // nothing: those keys take no part, and the device status word is set.
@@ -177,6 +181,8 @@ struct PagedCfg {
   static constexpr int CH = ROW / 16;                       // 16-byte chunks per row: 4, 8 or 16
   static constexpr int STAGES = 24576 / STAGE;              // 192 KB in all
   static constexpr int THREADS = WARPS * 32;
+  // the base lies BELOW binary places below the maximum and moves when a score is TOP places above it
+  static constexpr float BELOW = FP8 ? 15.f : 0.f, TOP = FP8 ? 15.f : 8.f;
   static constexpr int RING = WARPS * STAGES * STAGE;
   // byte offset of chunk c of row r: 128-byte lines whose 16-byte chunks are
   // permuted so that the 8 rows ldmatrix reads at once hit 8 different chunks
@@ -406,12 +412,12 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
       for (int n = 0; n < KS; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[h][n][i] = 0.f;
-    float mx[HT][2], sum[HT][2];
+    float base2[HT][2], sum[HT][2];
 #pragma unroll
     for (int h = 0; h < HT; ++h)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        mx[h][j] = -INFINITY;
+        base2[h][j] = -INFINITY;
         sum[h][j] = 0.f;
       }
 #pragma unroll 1
@@ -462,19 +468,22 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
           for (int j = 0; j < 2; ++j) {
             s[h][j] = ok0 ? s[h][j] * sl2[h][j] : -INFINITY;
             s[h][2 + j] = ok1 ? s[h][2 + j] * sl2[h][j] : -INFINITY;
-            grew |= fmaxf(s[h][j], s[h][2 + j]) > mx[h][j] + 8.f;
+            grew |= fmaxf(s[h][j], s[h][2 + j]) - base2[h][j] > C::TOP;
           }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
           for (int h = 0; h < HT; ++h)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float nm = fmaxf(mx[h][j], fmaxf(s[h][j], s[h][2 + j]));
-              nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, 4));
-              nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, 8));
-              nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, 16));
-              const float f = nm > mx[h][j] ? ex2_approx(mx[h][j] - nm) : 1.f;  // 2^-inf = 0: nothing summed yet
-              mx[h][j] = nm;
+              float top = fmaxf(s[h][j], s[h][2 + j]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              float nb = top - C::BELOW;
+              if (top - nb > C::TOP) nb = top;  // scores so large that the difference is rounded
+              nb = fmaxf(nb, base2[h][j]);
+              const float f = nb > base2[h][j] ? ex2_approx(base2[h][j] - nb) : 1.f;  // 2^-inf = 0: nothing summed yet
+              base2[h][j] = nb;
               sum[h][j] *= f;
 #pragma unroll
               for (int n = 0; n < KS; ++n) {
@@ -486,7 +495,8 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
         uint32_t pb[HT][2];
 #pragma unroll
         for (int h = 0; h < HT; ++h) {
-          const float m0 = mx[h][0] == -INFINITY ? 0.f : mx[h][0], m1 = mx[h][1] == -INFINITY ? 0.f : mx[h][1];
+          const float m0 = base2[h][0] == -INFINITY ? 0.f : base2[h][0];
+          const float m1 = base2[h][1] == -INFINITY ? 0.f : base2[h][1];
           const float e00 = ex2_approx(s[h][0] - m0), e01 = ex2_approx(s[h][1] - m1);
           const float e10 = ex2_approx(s[h][2] - m0), e11 = ex2_approx(s[h][3] - m1);
           sum[h][0] += e00 + e10;
@@ -525,7 +535,7 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
     cp_async_wait<0>();
     __syncthreads();  // the rings are free: they take the warps' results
 
-    // the warps' results -> shared memory: rows, maxima, sums
+    // the warps' results -> shared memory: rows, bases (as maxima below), sums
     float* mg = reinterpret_cast<float*>(paged_sm);
     float* mg_m = mg + W * R * D;
     float* mg_l = mg_m + W * R;
@@ -539,7 +549,7 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int row = 8 * h + 2 * t4 + j;
         if (g == 0) {
-          mg_m[warp * R + row] = mx[h][j];
+          mg_m[warp * R + row] = base2[h][j];
           mg_l[warp * R + row] = l;
         }
         float* dst = mg + (warp * R + row) * D;

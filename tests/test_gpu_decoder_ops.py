@@ -635,6 +635,53 @@ def test_attention_paged_large_queries_fp8():
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("lens,hq,hk,D,page", [
+    ([20000], 4, 1, 128, 16),              # one sequence over many SMs
+    ([9000, 33, 6000] + [700] * 40, 8, 4, 64, 64),
+    ([500] * 300, 12, 1, 128, 32),         # whole sequences in one range, 9 to 16 heads
+])
+@pytest.mark.parametrize("nats,spread", [(3, 0.3), (12, 0.3), (15, 0.0), (16.9, 0.0), (17.5, 0.3), (19, 0.3), (20, 0.0), (30, 0.0)])
+def test_attention_paged_sinks(kind, lens, hq, hk, D, page, nats, spread):
+    """A token that outweighs all others and whose value is zero: the output is made of the others' small
+    probabilities.  Over an E4M3 cache they are fp16 above a base 2^-15 of the largest: half a step is 2^-11 of the value
+    or 2^-25 2^-15, whichever is more, so a probability is off by 2^-40 at most where it is below fp16's normal range."""
+    g = gen(sum(lens) + D + int(nats * 10))
+    n = [-(-m // page) for m in lens]
+    sign = (torch.randint(0, 2, (hk, D), generator=g) * 2 - 1).float()
+    q = sign.repeat_interleave(hq // hk, 0).reshape(1, -1).expand(len(lens), -1).to(BF).to(DEV).contiguous()
+    # rest: scores of standard deviation ``spread`` nats below the sink's
+    scale = nats / D
+    kc = torch.randn(sum(n), page, hk, D, generator=g) * (spread / (scale * D ** 0.5))
+    vc = torch.randn(sum(n), page, hk, D, generator=g)
+    table = torch.zeros(len(lens), max(n), dtype=torch.int32)
+    at = 0
+    for b, m in enumerate(n):
+        table[b, :m] = torch.arange(at, at + m)
+        at += m
+    for b, m in enumerate(lens):
+        t = int(torch.randint(0, m, (1,), generator=g))
+        kc[table[b, t // page], t % page] = sign
+        vc[table[b, t // page], t % page] = 0
+    kc, vc, table = kc.to(DEV), vc.to(DEV), table.to(DEV)
+    kw = {}
+    if kind == "fp8":
+        kc, vc = (c.to(torch.float8_e4m3fn).view(torch.uint8) for c in (kc, vc))
+        kw = {"k_scale": torch.ones(hk, device=DEV), "v_scale": torch.ones(hk, device=DEV)}
+    else:
+        kc, vc = kc.to(BF), vc.to(BF)
+    lse = torch.empty(len(lens), hq, device=DEV)
+    o = K.attention_paged(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device=DEV), scale=scale, lse=lse, **kw)
+    some = [0, 1, 2, len(lens) - 1] if len(lens) > 3 else range(len(lens))  # sequences that are looked at
+    want, tol, wl = paged_ref(q[some], kc, vc, table[some], [lens[b] for b in some], kw.get("k_scale"), kw.get("v_scale"),
+                              scale, kind)
+    if kind == "fp8":
+        top = e4m3_value(vc).abs().max()
+        tol = tol + torch.tensor([[lens[b]] for b in some], device=DEV) * 2.0 ** -40 * top
+    assert ((o[some].double() - want).abs() <= tol).all(), ((o[some].double() - want).abs() / tol).max().item()
+    close_lse(lse[some], wl)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
 def test_attention_paged_garbage_behind_the_length(kind):
     """Slots behind a sequence's last token hold NaN (bf16 and E4M3 have one): the result does not see them."""
     g = gen(6)
