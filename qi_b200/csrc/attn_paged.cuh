@@ -387,9 +387,9 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
       if (FP8) {
         qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, 1));
         qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, 2));
-        // 2^e with e the exponent of the row's largest element, kept so that 2^-e is a normal number
-        int e = static_cast<int>(__float_as_uint(qmax) >> 23) - 127;
-        e = max(-100, min(100, e));
+        // the row's largest element goes to fp16's last binade (at most 255 2^8 there), so that
+        // small ones beside it keep their bits down to 2^-29 of it; both powers stay normal
+        const int e = max(-126, static_cast<int>(__float_as_uint(qmax) >> 23) - 127 - 15);
         up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
         const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll

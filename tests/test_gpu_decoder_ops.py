@@ -634,6 +634,35 @@ def test_attention_paged_large_queries_fp8():
     assert ((o.double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("outlier", [0, 12, 17, 22, 26])
+@pytest.mark.parametrize("mul,scale", [(1.0, None), (1e-30, 1e29), (1e36, 1e-37)])
+def test_attention_paged_queries_of_many_magnitudes_fp8(outlier, mul, scale):
+    """A column of q that is 2^outlier times the others, where the keys are zero: the scores are those of the other
+    columns.  In fp16 the row's largest element lies in its last binade, [2^15, 2^16), and half a step of its smallest
+    numbers is 2^-25: an element is off by 2^-40 of the largest at most where 2^-11 of itself is not more; bf16's 8 bits
+    fit where it is above 2^-14, so the rest is exact."""
+    g = gen(outlier + int(mul < 1))
+    lens = [700, 64]
+    table, kc, vc, (ks, vs) = make_cache(g, lens, 16, 2, 128, "fp8", "token")
+    q = randn(g, 2, 4 * 128)
+    q = (q.double() * (mul if outlier == 0 or mul <= 1 else mul * 2.0 ** -outlier)).to(BF)
+    q[:, 5::128] = (q[:, 6::128].double() * 2.0 ** outlier).to(BF)
+    if mul > 1 and outlier:
+        scale = scale * 2.0 ** outlier
+    if outlier:
+        kc[..., 5] = 0
+    scale = scale or 128 ** -0.5
+    o = K.attention_paged(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device=DEV), k_scale=ks, v_scale=vs,
+                          scale=scale)
+    want, tol, _ = paged_ref(q, kc, vc, table, lens, ks, vs, scale, "fp8")
+    most = (e4m3_value(kc.contiguous()).abs() * ks.double()[:, None]).nan_to_num().sum(-1).max()
+    top = q.double().abs().max()
+    values = e4m3_value(vc.contiguous()).abs().max() * vs.max()
+    tol = tol + 2 * 2.0 ** -40 * top * most * scale * values
+    assert torch.isfinite(o).all()
+    assert ((o.double() - want).abs() <= tol).all(), ((o.double() - want).abs() / tol).max().item()
+
+
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
 @pytest.mark.parametrize("lens,hq,hk,D,page", [
     ([20000], 4, 1, 128, 16),              # one sequence over many SMs
