@@ -266,7 +266,8 @@ int qi_b200_attention_short(const void* q, long long ldq, const void* k, long lo
  *   KIND_BF16: no codes (q, scales unused)
  * xn (optional with codes, required with KIND_BF16) receives bf16(v).
  * q [M, D] and xn [M, D] are dense; D % 8 == 0, D <= 16384.  A row that holds
- * an infinity or NaN gets the scale NaN. */
+ * an infinity or NaN, in h or in the weight, gets the scale NaN, and so does one
+ * whose sum of h^2 or whose h * weight passes fp32's range (|h| of 1e17 and more). */
 int qi_b200_rms_norm_quant(int kind, const void* x_bf16, long long ldx, const void* y_bf16, long long ldy,
                            void* x_out_bf16, long long ld_out, const void* weight_bf16, void* q, float* scales,
                            void* xn_bf16, int M, int D, float eps, cudaStream_t stream);

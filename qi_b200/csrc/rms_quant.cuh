@@ -63,6 +63,13 @@ __device__ __forceinline__ uint32_t rms_codes4(float a, float b, float c, float 
   }
 }
 
+// The larger one; NaN where either is one (fmaxf drops it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // T threads per row (whole warps, at most 512), blockDim.x / T rows per CTA,
 // C chunks of 8 elements per thread.  FMT: 0 bf16 only, 1 INT8, 2 E4M3.
 template <int C, int FMT>
@@ -110,13 +117,13 @@ __global__ void __launch_bounds__(512) k_rms_quant(const RmsQuantParams p, int T
     for (int e = 0; e < 4; ++e) {
       ss = fmaf(f[e].x, f[e].x, ss);
       ss = fmaf(f[e].y, f[e].y, ss);
-      mx = fmaxf(mx, fmaxf(fabsf(f[e].x * w[e].x), fabsf(f[e].y * w[e].y)));
+      mx = max_nan(mx, max_nan(fabsf(f[e].x * w[e].x), fabsf(f[e].y * w[e].y)));
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
   if (T > 32) {
     if (lane == 0) red[warp] = make_float2(ss, mx);
@@ -126,12 +133,15 @@ __global__ void __launch_bounds__(512) k_rms_quant(const RmsQuantParams p, int T
     for (int w = 0; w < (T >> 5); ++w) {
       const float2 v = red[w0 + w];
       ss += v.x;
-      mx = fmaxf(mx, v.y);
+      mx = max_nan(mx, v.y);
     }
   }
   const float r = rsqrtf(ss / static_cast<float>(p.D) + p.eps);
-  // a row with an infinity or NaN has no scale: NaN, as the maximum of its values is
-  const float amax = ss < __int_as_float(0x7f800000) ? mx * r : __int_as_float(0x7fffffff);
+  // a row with an infinity or NaN, its own or the weight's, has no scale: NaN (h w is one
+  // of the two wherever h or w is), and so has one whose sum of squares or product is
+  // beyond fp32
+  constexpr float kInf = __builtin_huge_valf();
+  const float amax = ss < kInf && mx < kInf ? mx * r : __int_as_float(0x7fffffff);
   float s = 1.f;
   if (FMT == 1) s = amax == amax ? fmaxf(__fdiv_rn(amax, 127.0f), 1e-10f) : amax;
   if (FMT == 2) s = amax == amax ? fmaxf(__fdiv_rn(amax, 448.0f), 1e-12f) : amax;

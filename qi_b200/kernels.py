@@ -574,7 +574,9 @@ def rms_norm_quant(kind: int, x: torch.Tensor, weight: torch.Tensor, y: torch.Te
     ``KIND_INT8`` returns (int8 [M, D], fp32 [M]), ``KIND_FP8_E4M3`` (uint8
     E4M3 codes [M, D], fp32 [M]), the operands of ``gemm``; ``KIND_BF16``
     returns (None, None) and needs ``xn``.  ``xn`` [M, D] receives the
-    normalized row in bf16.  D % 8 == 0, D <= 16384."""
+    normalized row in bf16.  A row with an infinity or NaN in it or in
+    ``weight``, or whose squares pass fp32's range, gets the scale NaN.
+    D % 8 == 0, D <= 16384."""
     return _op("rms_norm_quant", kind, x, weight, y, eps, x_out, q, s, xn)
 
 

@@ -155,6 +155,33 @@ def test_rms_norm_quant_zero_and_non_finite_rows(kind):
     assert torch.isfinite(s[[0, 4]]).all() and torch.equal(q[0], q[4])
 
 
+@pytest.mark.parametrize("kind", [_lib.KIND_INT8, _lib.KIND_FP8_E4M3])
+@pytest.mark.parametrize("M,D", [(3, 64), (5, 4096), (300, 8192)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_rms_norm_quant_non_finite_weight(kind, M, D, what):
+    """An infinity or a NaN in the weight is in a value of every row: no row has a scale."""
+    g = gen(M + D)
+    x, w = randn(g, M, D), randn(g, D)
+    x[0] = 0
+    w[D - 3] = what
+    xn = torch.empty_like(x)
+    q, s = K.rms_norm_quant(kind, x, w, xn=xn)
+    assert torch.isnan(s).all()
+    assert not torch.isfinite(xn[1:, D - 3]).any()
+
+
+@pytest.mark.parametrize("kind", [_lib.KIND_INT8, _lib.KIND_FP8_E4M3])
+def test_rms_norm_quant_rows_beyond_fp32(kind):
+    """Finite rows whose sum of squares passes fp32's range have no scale; rows in front of it have theirs."""
+    x = torch.full((3, 512), 1e17, dtype=BF, device=DEV)
+    x[1] = 2e18  # 512 * 4e36 > 3.4e38
+    w = torch.full((512,), 0.5, dtype=BF, device=DEV)
+    q, s = K.rms_norm_quant(kind, x, w)
+    assert torch.isnan(s[1]) and torch.isfinite(s[[0, 2]]).all()
+    keep = torch.tensor([0, 2], device=DEV)
+    check_norm(kind, None, w, None, 1e-6, q[keep], s[keep], x[keep])
+
+
 # ---------------------------------------------------------------------------
 # rope_axes
 # ---------------------------------------------------------------------------
