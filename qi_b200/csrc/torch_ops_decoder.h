@@ -322,28 +322,139 @@ inline at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_cache
   return o;
 }
 
+// ---------------------------------------------------------------------------
+// The forms that qi_b200.kernels calls: `fresh` returns new tensors only, `out`
+// writes given ones and returns nothing, so that what a call writes and what it
+// returns never are one tensor (tracers rely on it).  The forms without an
+// overload name take either and may return an argument.
+
+inline std::tuple<at::Tensor, at::Tensor> rms_norm_quant_fresh(int64_t kind, const at::Tensor& x,
+                                                               const at::Tensor& weight, const Opt& y, double eps,
+                                                               const Opt& x_out, const Opt& xn) {
+  TORCH_CHECK_VALUE(kind != QI_B200_KIND_BF16, "KIND_BF16 has no codes.");
+  TORCH_CHECK_VALUE(!given(y) || given(x_out), "y needs x_out.");
+  auto r = rms_norm_quant(kind, x, weight, y, eps, x_out, {}, {}, xn);
+  return {*std::get<0>(r), *std::get<1>(r)};
+}
+inline void rms_norm_quant_out(int64_t kind, const at::Tensor& x, const at::Tensor& weight, const Opt& y, double eps,
+                               const Opt& x_out, const Opt& q, const Opt& s, const Opt& xn) {
+  TORCH_CHECK_VALUE(!given(y) || given(x_out), "y needs x_out.");
+  TORCH_CHECK_VALUE(kind == QI_B200_KIND_BF16 || (given(q) && given(s)), "codes need q and s.");
+  rms_norm_quant(kind, x, weight, y, eps, x_out, q, s, xn);
+}
+
+inline std::tuple<at::Tensor, at::Tensor> rope_axes_fresh(const at::Tensor& q, const Opt& k, const at::Tensor& positions,
+                                                          const at::Tensor& freqs, const at::Tensor& axes,
+                                                          int64_t head_dim, bool interleaved) {
+  auto r = rope_axes(q, k, positions, freqs, axes, head_dim, interleaved, {}, {});
+  const Opt& ok = std::get<1>(r);
+  return {std::get<0>(r), given(ok) ? *ok : at::empty({0}, q.options())};
+}
+inline void rope_axes_out(const at::Tensor& q, const Opt& k, const at::Tensor& positions, const at::Tensor& freqs,
+                          const at::Tensor& axes, int64_t head_dim, bool interleaved, const at::Tensor& out_q,
+                          const Opt& out_k) {
+  TORCH_CHECK_VALUE(given(k) == given(out_k), given(k) ? "k needs out_k." : "out_k needs k.");
+  rope_axes(q, k, positions, freqs, axes, head_dim, interleaved, out_q, out_k);
+}
+
+inline at::Tensor rope_axes_store_fresh(const at::Tensor& q, const Opt& k, const Opt& v, const at::Tensor& positions,
+                                        const at::Tensor& freqs, const at::Tensor& axes, int64_t head_dim,
+                                        const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& slots,
+                                        bool interleaved, const Opt& k_scale, const Opt& v_scale, const Opt& out_k) {
+  return rope_axes_store(q, k, v, positions, freqs, axes, head_dim, k_cache, v_cache, slots, interleaved, k_scale,
+                         v_scale, {}, out_k);
+}
+inline void rope_axes_store_out(const at::Tensor& q, const Opt& k, const Opt& v, const at::Tensor& positions,
+                                const at::Tensor& freqs, const at::Tensor& axes, int64_t head_dim,
+                                const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& slots,
+                                bool interleaved, const Opt& k_scale, const Opt& v_scale, const at::Tensor& out_q,
+                                const Opt& out_k) {
+  rope_axes_store(q, k, v, positions, freqs, axes, head_dim, k_cache, v_cache, slots, interleaved, k_scale, v_scale,
+                  out_q, out_k);
+}
+
+inline at::Tensor attention_packed_fresh(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                         const at::Tensor& cu_q, const at::Tensor& cu_k, int64_t heads,
+                                         int64_t kv_heads, bool causal, std::optional<double> scale, const Opt& lse) {
+  return attention_packed(q, k, v, cu_q, cu_k, heads, kv_heads, causal, scale, {}, lse);
+}
+inline void attention_packed_out(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q,
+                                 const at::Tensor& cu_k, int64_t heads, int64_t kv_heads, bool causal,
+                                 std::optional<double> scale, const at::Tensor& out, const Opt& lse) {
+  attention_packed(q, k, v, cu_q, cu_k, heads, kv_heads, causal, scale, out, lse);
+}
+
+inline at::Tensor attention_paged_fresh(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                        const at::Tensor& pages, const at::Tensor& lengths,
+                                        std::optional<double> scale, const Opt& k_scale, const Opt& v_scale,
+                                        const Opt& lse) {
+  return attention_paged(q, k_cache, v_cache, pages, lengths, scale, k_scale, v_scale, {}, lse);
+}
+inline void attention_paged_out(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                const at::Tensor& pages, const at::Tensor& lengths, std::optional<double> scale,
+                                const Opt& k_scale, const Opt& v_scale, const at::Tensor& out, const Opt& lse) {
+  attention_paged(q, k_cache, v_cache, pages, lengths, scale, k_scale, v_scale, out, lse);
+}
+
 }  // namespace decoder
 
 TORCH_LIBRARY_FRAGMENT(qi_b200, m) {
   m.def("rms_norm_quant(int kind, Tensor(a!) x, Tensor weight, Tensor? y=None, float eps=1e-6, Tensor(b!)? x_out=None, "
-        "Tensor(c!)? q=None, Tensor(d!)? s=None, Tensor(e!)? xn=None) -> (Tensor?, Tensor?)");
+        "Tensor(c!)? q=None, Tensor(d!)? s=None, Tensor(e!)? xn=None) -> (Tensor(c!)?, Tensor(d!)?)");
+  m.def("rms_norm_quant.fresh(int kind, Tensor x, Tensor weight, Tensor? y, float eps, Tensor(a!)? x_out, "
+        "Tensor(b!)? xn) -> (Tensor, Tensor)");
+  m.def("rms_norm_quant.out(int kind, Tensor x, Tensor weight, Tensor? y, float eps, Tensor(a!)? x_out, "
+        "Tensor(b!)? q, Tensor(c!)? s, Tensor(d!)? xn) -> ()");
   m.def("rope_axes(Tensor q, Tensor? k, Tensor positions, Tensor freqs, Tensor axes, int head_dim, "
-        "bool interleaved=True, Tensor(a!)? out_q=None, Tensor(b!)? out_k=None) -> (Tensor, Tensor?)");
+        "bool interleaved=True, Tensor(a!)? out_q=None, Tensor(b!)? out_k=None) -> (Tensor(a!), Tensor(b!)?)");
+  m.def("rope_axes.fresh(Tensor q, Tensor? k, Tensor positions, Tensor freqs, Tensor axes, int head_dim, "
+        "bool interleaved) -> (Tensor, Tensor)");
+  m.def("rope_axes.out(Tensor q, Tensor? k, Tensor positions, Tensor freqs, Tensor axes, int head_dim, "
+        "bool interleaved, Tensor(a!) out_q, Tensor(b!)? out_k) -> ()");
   m.def("rope_axes_store(Tensor q, Tensor? k, Tensor? v, Tensor positions, Tensor freqs, Tensor axes, int head_dim, "
         "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, bool interleaved=True, Tensor? k_scale=None, "
-        "Tensor? v_scale=None, Tensor(c!)? out_q=None, Tensor(d!)? out_k=None) -> Tensor");
+        "Tensor? v_scale=None, Tensor(c!)? out_q=None, Tensor(d!)? out_k=None) -> Tensor(c!)");
+  m.def("rope_axes_store.fresh(Tensor q, Tensor? k, Tensor? v, Tensor positions, Tensor freqs, Tensor axes, "
+        "int head_dim, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, bool interleaved, Tensor? k_scale, "
+        "Tensor? v_scale, Tensor(c!)? out_k) -> Tensor");
+  m.def("rope_axes_store.out(Tensor q, Tensor? k, Tensor? v, Tensor positions, Tensor freqs, Tensor axes, "
+        "int head_dim, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, bool interleaved, Tensor? k_scale, "
+        "Tensor? v_scale, Tensor(c!) out_q, Tensor(d!)? out_k) -> ()");
   m.def("attention_packed(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k, int heads, int kv_heads, "
-        "bool causal=True, float? scale=None, Tensor(a!)? out=None, Tensor(b!)? lse=None) -> Tensor");
+        "bool causal=True, float? scale=None, Tensor(a!)? out=None, Tensor(b!)? lse=None) -> Tensor(a!)");
+  m.def("attention_packed.fresh(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k, int heads, int kv_heads, "
+        "bool causal, float? scale, Tensor(a!)? lse) -> Tensor");
+  m.def("attention_packed.out(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k, int heads, int kv_heads, "
+        "bool causal, float? scale, Tensor(a!) out, Tensor(b!)? lse) -> ()");
   m.def("attention_paged(Tensor q, Tensor k_cache, Tensor v_cache, Tensor pages, Tensor lengths, float? scale=None, "
-        "Tensor? k_scale=None, Tensor? v_scale=None, Tensor(a!)? out=None, Tensor(b!)? lse=None) -> Tensor");
+        "Tensor? k_scale=None, Tensor? v_scale=None, Tensor(a!)? out=None, Tensor(b!)? lse=None) -> Tensor(a!)");
+  m.def("attention_paged.fresh(Tensor q, Tensor k_cache, Tensor v_cache, Tensor pages, Tensor lengths, float? scale, "
+        "Tensor? k_scale, Tensor? v_scale, Tensor(a!)? lse) -> Tensor");
+  m.def("attention_paged.out(Tensor q, Tensor k_cache, Tensor v_cache, Tensor pages, Tensor lengths, float? scale, "
+        "Tensor? k_scale, Tensor? v_scale, Tensor(a!) out, Tensor(b!)? lse) -> ()");
 }
 
-// One implementation for every backend: the checks come before the question
-// whether the tensors are CUDA's.
-TORCH_LIBRARY_IMPL(qi_b200, CompositeExplicitAutograd, m) {
-  m.impl("rms_norm_quant", &decoder::rms_norm_quant);
-  m.impl("rope_axes", &decoder::rope_axes);
-  m.impl("rope_axes_store", &decoder::rope_axes_store);
-  m.impl("attention_packed", &decoder::attention_packed);
-  m.impl("attention_paged", &decoder::attention_paged);
+// CPU tensors come to the same functions, whose checks refuse them (the checks
+// of types and shapes first).  Shapes without data are qi_b200/torch_ops.py's.
+namespace decoder {
+inline void register_all(torch::Library& m) {
+  m.impl("rms_norm_quant", &rms_norm_quant);
+  m.impl("rms_norm_quant.fresh", &rms_norm_quant_fresh);
+  m.impl("rms_norm_quant.out", &rms_norm_quant_out);
+  m.impl("rope_axes", &rope_axes);
+  m.impl("rope_axes.fresh", &rope_axes_fresh);
+  m.impl("rope_axes.out", &rope_axes_out);
+  m.impl("rope_axes_store", &rope_axes_store);
+  m.impl("rope_axes_store.fresh", &rope_axes_store_fresh);
+  m.impl("rope_axes_store.out", &rope_axes_store_out);
+  m.impl("attention_packed", &attention_packed);
+  m.impl("attention_packed.fresh", &attention_packed_fresh);
+  m.impl("attention_packed.out", &attention_packed_out);
+  m.impl("attention_paged", &attention_paged);
+  m.impl("attention_paged.fresh", &attention_paged_fresh);
+  m.impl("attention_paged.out", &attention_paged_out);
 }
+}  // namespace decoder
+
+TORCH_LIBRARY_IMPL(qi_b200, CUDA, m) { decoder::register_all(m); }
+TORCH_LIBRARY_IMPL(qi_b200, CPU, m) { decoder::register_all(m); }

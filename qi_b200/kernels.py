@@ -541,18 +541,29 @@ def fp8_linear(x_bf16_2d: torch.Tensor, weight_fp8: torch.Tensor, weight_scale: 
 # ---------------------------------------------------------------------------
 
 
-_OPS: dict = {}
 _STATUS = re.compile(r"^(\w+) failed with status (\d+)")
+_ready = False
 
 
-def _op(name: str, *args):
-    """Call the compiled torch operator ``qi_b200::<name>``, which checks the
-    arguments (``ValueError``), allocates and launches; a status of the library
-    comes back as the exceptions of ``_lib.check``."""
-    op = _OPS.get(name)
-    if op is None:
-        torch_ops.load()
-        op = _OPS[name] = getattr(torch.ops.qi_b200, name).default
+@torch.compiler.assume_constant_result
+def _load_ops() -> bool:
+    global _ready
+    torch_ops.load()
+    _ready = True
+    return True
+
+
+def _ops():
+    """The compiled torch operators of the decoder block.  They check the
+    arguments (``ValueError``), allocate and launch."""
+    if not _ready:
+        _load_ops()
+    return torch.ops.qi_b200
+
+
+def _call(op, *args):
+    """Call a compiled operator; a status of the library comes back as the
+    exceptions of ``_lib.check``."""
     try:
         return op(*args)
     except RuntimeError as e:
@@ -577,7 +588,18 @@ def rms_norm_quant(kind: int, x: torch.Tensor, weight: torch.Tensor, y: torch.Te
     normalized row in bf16.  A row with an infinity or NaN in it or in
     ``weight``, or whose squares pass fp32's range, gets the scale NaN.
     D % 8 == 0, D <= 16384."""
-    return _op("rms_norm_quant", kind, x, weight, y, eps, x_out, q, s, xn)
+    op = _ops().rms_norm_quant
+    if y is not None and x_out is None:
+        x_out = x
+    if q is None and s is None and kind != _lib.KIND_BF16:
+        return _call(op.fresh, kind, x, weight, y, eps, x_out, xn)
+    if kind != _lib.KIND_BF16:
+        if q is None:
+            q = x.new_empty(x.shape, dtype=torch.int8 if kind == _lib.KIND_INT8 else _U8)
+        if s is None:
+            s = x.new_empty(x.shape[:1], dtype=torch.float32)
+    _call(op.out, kind, x, weight, y, eps, x_out, q, s, xn)
+    return q, s
 
 
 def rope_axes_frequencies(sections, theta: float = 10000.0, shared: bool = False, device="cuda"):
@@ -610,7 +632,16 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, 
     (2i, 2i+1) (``interleaved``, as the DiT's) or (i, i + pairs); elements
     behind the last pair pass unchanged.  Returns (q, k) rotated; ``out_q`` /
     ``out_k`` may be ``q`` / ``k`` themselves."""
-    return _op("rope_axes", q, k, positions, freqs, axes, head_dim, interleaved, out_q, out_k)
+    op = _ops().rope_axes
+    if out_q is None and out_k is None:
+        out_q, out_k = _call(op.fresh, q, k, positions, freqs, axes, head_dim, interleaved)
+        return out_q, None if k is None else out_k
+    if out_q is None:
+        out_q = q.new_empty(q.shape)
+    if out_k is None and k is not None:
+        out_k = k.new_empty(k.shape)
+    _call(op.out, q, k, positions, freqs, axes, head_dim, interleaved, out_q, out_k)
+    return out_q, out_k
 
 
 def rope_axes_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor,
@@ -628,8 +659,13 @@ def rope_axes_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     [M]: page * page_size + place of each row, all different; a negative slot
     writes nothing (padding rows), one outside the cache writes nothing and is
     reported by ``_lib.raise_on_device_error``.  Returns the rotated q."""
-    return _op("rope_axes_store", q, k, v, positions, freqs, axes, head_dim, k_cache, v_cache, slots, interleaved,
-               k_scale, v_scale, out_q, out_k)
+    op = _ops().rope_axes_store
+    if out_q is None:
+        return _call(op.fresh, q, k, v, positions, freqs, axes, head_dim, k_cache, v_cache, slots, interleaved, k_scale,
+                     v_scale, out_k)
+    _call(op.out, q, k, v, positions, freqs, axes, head_dim, k_cache, v_cache, slots, interleaved, k_scale, v_scale,
+          out_q, out_k)
+    return out_q
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
@@ -645,7 +681,11 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     bf16 (or writes ``out``, which must not overlap the inputs; its rows
     outside every sequence stay as they were).  ``lse`` fp32 [Tq, heads] receives the log of the softmax sums.
     Default scale 1 / sqrt(D)."""
-    return _op("attention_packed", q, k, v, cu_q, cu_k, heads, kv_heads, causal, scale, out, lse)
+    op = _ops().attention_packed
+    if out is None:
+        return _call(op.fresh, q, k, v, cu_q, cu_k, heads, kv_heads, causal, scale, lse)
+    _call(op.out, q, k, v, cu_q, cu_k, heads, kv_heads, causal, scale, out, lse)
+    return out
 
 
 def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor,
@@ -663,4 +703,8 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     behind the table, is left out and reported by
     ``_lib.raise_on_device_error``.  Returns [B, heads * D] bf16 (or writes
     ``out``, which must not overlap the inputs); ``lse`` fp32 [B, heads] receives the log of the softmax sums."""
-    return _op("attention_paged", q, k_cache, v_cache, pages, lengths, scale, k_scale, v_scale, out, lse)
+    op = _ops().attention_paged
+    if out is None:
+        return _call(op.fresh, q, k_cache, v_cache, pages, lengths, scale, k_scale, v_scale, lse)
+    _call(op.out, q, k_cache, v_cache, pages, lengths, scale, k_scale, v_scale, out, lse)
+    return out

@@ -270,3 +270,108 @@ def test_packed_items_are_taken_once_longest_first(seed):
         assert [m[1] for m in mine] == sorted((m[1] for m in mine), reverse=True)
         seen += mine
     assert sorted(seen) == sorted((b, l, h) for b in range(len(lens)) for l in range(blocks[b]) for h in range(heads))
+
+
+# ---------------------------------------------------------------------------
+# tracing: results from shapes alone, and schemas that say what is written
+# ---------------------------------------------------------------------------
+
+OPS = ("rms_norm_quant", "rope_axes", "rope_axes_store", "attention_packed", "attention_paged")
+
+
+def decoder_calls(dev):
+    """(call, [(shape, dtype)] of its results) for every form of every operator; ``dev`` makes the tensors."""
+    e = lambda *shape, dtype=BF: torch.empty(*shape, dtype=dtype, device=dev)
+    i32, i64, f32 = torch.int32, torch.int64, torch.float32
+    x, w, f, a = e(4, 256), e(256), e(64, dtype=torch.float64), e(64, dtype=i32)
+    qkv = e(4, 512)
+    q, k, v = qkv.split([256, 128, 128], 1)
+    pos, slots = e(4, dtype=i32), e(4, dtype=i64)
+    kc, k8 = e(2, 4, 1, 128), e(2, 4, 1, 128, dtype=torch.uint8)
+    s1, cu, table, n = e(1, dtype=f32), e(2, dtype=i32), e(4, 2, dtype=i32), e(4, dtype=i32)
+    q8, s, lse = e(4, 256, dtype=torch.int8), e(4, dtype=f32), e(4, 2, dtype=f32)
+    row, kv = ((4, 256), BF), ((4, 128), BF)
+    i8, u8, sc = ((4, 256), torch.int8), ((4, 256), torch.uint8), ((4,), f32)
+    rope = lambda k=k, **kw: K.rope_axes(q, k, pos, f, a, 128, **kw)
+    store = lambda c=kc, **kw: K.rope_axes_store(q, k, v, pos, f, a, 128, c, c, slots, **kw)
+    packed = lambda **kw: K.attention_packed(q, k, v, cu, cu, 2, 1, **kw)
+    paged = lambda c=kc, **kw: K.attention_paged(q, c, c, table, n, **kw)
+    fp8 = dict(c=k8, k_scale=s1, v_scale=s1)
+    return [
+        (lambda: K.rms_norm_quant(I8, x, w), [i8, sc]),
+        (lambda: K.rms_norm_quant(FP8, x, w, q, x_out=e(4, 256)), [u8, sc]),
+        (lambda: K.rms_norm_quant(I8, x, w, q), [i8, sc]),
+        (lambda: K.rms_norm_quant(I8, x, w, q, q=q8), [i8, sc]),
+        (lambda: K.rms_norm_quant(I8, x, w, s=s, xn=e(4, 256)), [i8, sc]),
+        (lambda: K.rms_norm_quant(I8, x, w, q=q8, s=s), [i8, sc]),
+        (lambda: K.rms_norm_quant(BF16, x, w, xn=e(4, 256)), [None, None]),
+        (lambda: rope(), [row, kv]),
+        (lambda: rope(k=None), [row, None]),
+        (lambda: rope(out_q=q), [row, kv]),
+        (lambda: rope(out_k=k), [row, kv]),
+        (lambda: rope(out_q=q, out_k=k), [row, kv]),
+        (lambda: store(), [row]),
+        (lambda: store(out_q=q, out_k=k), [row]),
+        (lambda: store(out_k=k, **fp8), [row]),
+        (lambda: packed(), [row]),
+        (lambda: packed(lse=lse), [row]),
+        (lambda: packed(out=e(4, 256), lse=lse), [row]),
+        (lambda: paged(), [row]),
+        (lambda: paged(lse=lse, **fp8), [row]),
+        (lambda: paged(out=e(4, 256)), [row]),
+    ]
+
+
+def check_shapes(call, want, device):
+    got = call()
+    got = got if isinstance(got, tuple) else (got,)
+    assert [None if t is None else (tuple(t.shape), t.dtype) for t in got] == want
+    assert all(t is None or t.device.type == device for t in got)
+
+
+@pytest.mark.parametrize("i", range(21))
+def test_fake_and_meta_tensors(i):
+    """Tracing sees every form's results by shape, without data: fake CUDA tensors (as torch.compile makes them) and
+    meta tensors."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    assert len(decoder_calls("meta")) == 21
+    check_shapes(*decoder_calls("meta")[i], "meta")
+    with FakeTensorMode():
+        check_shapes(*decoder_calls("cuda")[i], "cuda")
+
+
+def test_fake_tensors_of_wrong_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        e = lambda *shape, dtype=BF: torch.empty(*shape, dtype=dtype, device="cuda")
+        f, a, i = e(64, dtype=torch.float64), e(64, dtype=torch.int32), e(4, dtype=torch.int32)
+        for call in (lambda: K.rms_norm_quant(I8, e(256), e(256)), lambda: K.rope_axes(e(4, 200), None, i, f, a, 128),
+                     lambda: K.attention_packed(e(4, 256), e(4, 256), e(4, 256), i, i, 3, 3),
+                     lambda: K.attention_paged(e(4, 256), e(2, 4, 128), e(2, 4, 128), e(4, 2), i)):
+            with pytest.raises(ValueError, match="must be"):
+                call()
+
+
+@pytest.mark.parametrize("name", OPS)
+def test_schemas_say_what_is_written_and_returned(name):
+    from qi_b200 import torch_ops
+
+    torch_ops.load()
+    packet = getattr(torch.ops.qi_b200, name)
+    assert sorted(packet.overloads()) == ["default", "fresh", "out"]
+    fresh, out = packet.fresh._schema, packet.out._schema
+    assert fresh.returns and all(r.alias_info is None for r in fresh.returns)
+    assert not out.returns
+    written = {"rms_norm_quant": {"x_out", "q", "s", "xn"}, "rope_axes": {"out_q", "out_k"},
+               "rope_axes_store": {"k_cache", "v_cache", "out_q", "out_k"}, "attention_packed": {"out", "lse"},
+               "attention_paged": {"out", "lse"}}[name]
+    mutable = lambda schema: {a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write}
+    assert mutable(out) == written and mutable(fresh) < written
+    # the form that takes either: what it returns may be the argument that it names
+    whole = packet.default._schema
+    sets = {a.name: a.alias_info.before_set for a in whole.arguments if a.alias_info is not None}
+    returned = [next(n for n, b in sets.items() if b == r.alias_info.before_set) for r in whole.returns]
+    assert returned == {"rms_norm_quant": ["q", "s"], "rope_axes": ["out_q", "out_k"], "rope_axes_store": ["out_q"],
+                        "attention_packed": ["out"], "attention_paged": ["out"]}[name]

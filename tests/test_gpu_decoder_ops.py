@@ -1047,3 +1047,81 @@ def test_decoder_block_prompt_then_tokens():
         same = K.attention_packed(q, torch.cat(ks), torch.cat(vs), cu([1] * 3), cu(total), hq, hk)
         assert ((same.double() - want).abs() <= tol).all()
         yt = K.int8_linear(o, wo, so)
+
+
+# ---------------------------------------------------------------------------
+# tracing
+# ---------------------------------------------------------------------------
+
+
+def test_operators_pass_torchs_checks():
+    """torch's own checks of every form: what the schema does not declare written is not, results alias nothing that is
+    not declared, and the traced shapes are the real ones."""
+    g = gen(21)
+    M, hq, hk, D, page = 12, 4, 2, 64, 4
+    x, w = randn(g, M, hq * D), randn(g, hq * D)
+    k, v = randn(g, M, hk * D), randn(g, M, hk * D)
+    freqs, axes = K.rope_axes_frequencies((D // 2,), device=DEV)
+    pos, slots = torch.arange(M, device=DEV), torch.arange(M, device=DEV)
+    kc, vc = (randn(g, 3 * page, hk * D).view(3, page, hk, D) for _ in range(2))
+    c = cu([5, 7])
+    table, n = torch.tensor([[2, 0, 1]] * M, dtype=torch.int32, device=DEV), torch.full((M,), 9, dtype=torch.int32, device=DEV)
+    new = lambda t: torch.empty_like(t)
+    q8, s8 = torch.empty(M, hq * D, dtype=torch.int8, device=DEV), torch.empty(M, device=DEV)
+    lse = torch.empty(M, hq, device=DEV)
+    ops = torch.ops.qi_b200
+    K.rms_norm_quant(_lib.KIND_INT8, x, w)  # registers the operators
+    rope, store = (x, k, pos, freqs, axes, D, False), (x, k, v, pos, freqs, axes, D, kc, vc, slots, False, None, None)
+    packed, paged = (x, k, v, c, c, hq, hk, True, None), (x, kc, vc, table, n, None, None, None)
+    for op, args in [
+        (ops.rms_norm_quant.fresh, (0, x, w, None, 1e-6, None, new(x))),
+        (ops.rms_norm_quant.fresh, (1, x, w, k.repeat(1, 2), 1e-6, new(x), None)),
+        (ops.rms_norm_quant.out, (0, x, w, None, 1e-6, None, q8, s8, None)),
+        (ops.rms_norm_quant.default, (0, x, w, None, 1e-6, None, q8, None, None)),
+        (ops.rope_axes.fresh, rope), (ops.rope_axes.out, rope + (new(x), new(k))),
+        (ops.rope_axes.default, rope + (new(x), None)),
+        (ops.rope_axes_store.fresh, store + (None,)), (ops.rope_axes_store.out, store + (new(x), new(k))),
+        (ops.rope_axes_store.default, store + (new(x), None)),
+        (ops.attention_packed.fresh, packed + (lse,)), (ops.attention_packed.out, packed + (new(x), None)),
+        (ops.attention_packed.default, packed + (new(x), None)),
+        (ops.attention_paged.fresh, paged + (lse,)), (ops.attention_paged.out, paged + (new(x), None)),
+        (ops.attention_paged.default, paged + (new(x), None)),
+    ]:
+        torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_operators_in_a_compiled_function(dynamic):
+    """A decoder step traced as one graph (no breaks) gives the eager step's results, caches and residual stream."""
+    g = gen(22)
+    hq, hk, D, page = 4, 2, 64, 16
+    w = randn(g, hq * D)
+    wq = randn(g, hq * D, (hq + 2 * hk) * D, mul=0.05)
+    freqs, axes = K.rope_axes_frequencies((D // 2,), device=DEV)
+
+    def step(x, y, kc, vc, pos, slots, c, table, n):
+        xn = torch.empty_like(x)
+        q8, s8 = K.rms_norm_quant(_lib.KIND_FP8_E4M3, x, w, y, xn=xn)
+        q, k, v = (xn @ wq).split([hq * D, hk * D, hk * D], 1)
+        q2, k2 = K.rope_axes(q, k, pos, freqs, axes, D)
+        K.rope_axes_store(q, k, v, pos, freqs, axes, D, kc, vc, slots, out_q=q, out_k=k)
+        a = K.attention_packed(q, k, v, c, c, hq, hk)
+        b = K.attention_paged(q, kc, vc, table, n)
+        return q8, s8, q2, k2, a, b + a
+
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True, dynamic=dynamic)
+    for T in (40, 56):
+        x, y = randn(g, T, hq * D), randn(g, T, hq * D)
+        pages = -(-T // page)
+        state = [randn(g, pages * page, hk * D).view(pages, page, hk, D) for _ in range(2)]
+        pos = torch.arange(T, device=DEV)
+        rest = (pos, torch.randperm(pages * page, generator=g)[:T].to(DEV), cu([T - 9, 9]),
+                torch.randint(0, pages, (T, pages), generator=g).to(torch.int32).to(DEV),
+                torch.randint(1, T, (T,), generator=g).to(torch.int32).to(DEV))
+        runs = []
+        for fn in (compiled, step):
+            mine = [t.clone() for t in (x, y, *state)]
+            out = fn(*mine, *rest)
+            runs.append([*out, *mine])
+        for i, (a, b) in enumerate(zip(*runs)):
+            assert torch.equal(a, b), i
