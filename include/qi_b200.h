@@ -310,23 +310,27 @@ int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk
 
 /* Attention over packed sequences: rows cu_q[b] .. cu_q[b+1] of q attend the
  * rows cu_k[b] .. cu_k[b+1] of k and v (cu_* int32 [n_seq + 1], device,
- * ascending); with causal, query i of a sequence sees the keys
+ * ascending); with ATTN_CAUSAL, query i of a sequence sees the keys
  * j <= i + (lk - lq).  A query that sees no key gives zeros.  Query head h
- * reads key head h / (heads / kv_heads).  head_dim 64 or 128.  bf16 in and
+ * reads key head h / (heads / kv_heads).  head_dim 64 or 128.  flags: a sum of
+ * QI_B200_ATTN_CAUSAL and QI_B200_ATTN_ZERO_REST.  bf16 in and
  * out, fp32 scores and sums, probabilities rounded to bf16 before the product
  * with V.  lse (optional, fp32 [total_q, heads]): log of the sum of
  * exp(scale q.k), -inf where no key is seen.  Rows of out (and lse) outside
- * every sequence are left as they were.  An infinity or a NaN reaches the
+ * every sequence are left as they were, but those of out become zeros with
+ * QI_B200_ATTN_ZERO_REST.  An infinity or a NaN reaches the
  * queries that see it and no others.  out must not overlap the inputs.  With a workspace of the size that
  * qi_b200_attention_packed_workspace_bytes names (0: none is of use), items
  * may be cut over several SMs where they do not fill the device evenly; it
  * needs no initialization and may be used again by the next call on the
  * stream.  Without one (null, or smaller) nothing is cut. */
+#define QI_B200_ATTN_CAUSAL 1
+#define QI_B200_ATTN_ZERO_REST 2
 int qi_b200_attention_packed_workspace_bytes(int n_seq, int total_q, int total_k, int heads, int kv_heads, int head_dim,
                                              size_t* bytes);
 int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
                              void* out, long long ldo, float* lse, const int* cu_q, const int* cu_k, int n_seq,
-                             int total_q, int total_k, int heads, int kv_heads, int head_dim, int causal, float scale,
+                             int total_q, int total_k, int heads, int kv_heads, int head_dim, int flags, float scale,
                              void* workspace, size_t workspace_bytes, cudaStream_t stream);
 
 /* Attention of one new token per sequence over a paged cache: row b of q

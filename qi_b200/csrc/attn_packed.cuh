@@ -20,7 +20,8 @@
 // maximum rarely grows.
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of tile 0 and 1, warp 8 TMA,
-// warp 9 MMA, warp 10 the list of items (11 fills up the warpgroup).  A softmax
+// warp 9 MMA, warp 10 the list of items, warp 11 zeros for the rows outside every
+// sequence where they are asked for.  A softmax
 // thread holds a whole row of S, so the softmax warpgroups take 208 registers a
 // thread and the third leaves them all but 88 (of 168 at launch: 256 x 208 +
 // 128 x 88 = 64,512, all of them).  CTAs are persistent; each takes every
@@ -78,6 +79,7 @@ struct PackedParams {
   int heads, kv_heads, group;
   int pair_heads;    // 1: an item is two heads x 128 tokens, 0: one head x 256 tokens
   int causal;
+  int zero_rest;     // 1: rows of out outside every sequence become zeros
   float scale_log2e;
   __nv_bfloat16* out;
   long long ldo;
@@ -586,6 +588,16 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         ++n_it;
         return true;
       });
+    } else if (warp == 11) {
+      // ---- rows in front of the first sequence and behind the last ----
+      if (p.zero_rest) {
+        const int front = min(max(p.cu_q[0], 0), p.total_q), back = min(max(p.cu_q[p.n_seq], front), p.total_q);
+        const int width = p.heads * (D / 8);
+        for (int r = blockIdx.x; r < front + p.total_q - back; r += gridDim.x) {
+          uint4* to = reinterpret_cast<uint4*>(p.out + static_cast<long long>(r < front ? r : back + r - front) * p.ldo);
+          for (int i = lane; i < width; i += 32) to[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
     } else if (warp == 8) {
       // ---- TMA ----
       int stage = 0, issued = 0;

@@ -262,11 +262,13 @@ int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk
 
 int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
                              void* out, long long ldo, float* lse, const int* cu_q, const int* cu_k, int n_seq,
-                             int total_q, int total_k, int heads, int kv_heads, int head_dim, int causal, float scale,
+                             int total_q, int total_k, int heads, int kv_heads, int head_dim, int flags, float scale,
                              void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   if (head_dim != 64 && head_dim != 128) return QI_B200_ESHAPE;
   if (n_seq < 0 || total_q < 0 || total_k < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return QI_B200_ESHAPE;
-  if (n_seq == 0 || total_q == 0) return QI_B200_OK;
+  if (flags & ~(QI_B200_ATTN_CAUSAL | QI_B200_ATTN_ZERO_REST)) return QI_B200_EINVAL;
+  const bool zero_rest = (flags & QI_B200_ATTN_ZERO_REST) != 0;
+  if (total_q == 0 || (n_seq == 0 && !zero_rest)) return QI_B200_OK;
   if (static_cast<long long>(total_q) + total_k > 0x3fffffff) return QI_B200_ETOOBIG;  // key places in 32 bits
   if (q == nullptr || out == nullptr || cu_q == nullptr || cu_k == nullptr || (total_k > 0 && (!k || !v)))
     return QI_B200_EINVAL;
@@ -278,6 +280,8 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
   if (workspace != nullptr && !aligned16(workspace)) return QI_B200_EALIGN;
   DeviceInfo* di = nullptr;
   if (int rc = device_info(&di)) return rc;
+  if (n_seq == 0)
+    return cudaMemset2DAsync(out, ldo * 2, 0, wq * 2, total_q, stream) == cudaSuccess ? QI_B200_OK : QI_B200_ECUDA;
   const size_t need = packed_workspace(n_seq, total_q, total_k, heads, kv_heads, head_dim, di->num_sms);
   PackedParams p = {};
   p.ws = need > 0 && workspace != nullptr && workspace_bytes >= need ? static_cast<float*>(workspace) : nullptr;
@@ -290,7 +294,8 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
   p.kv_heads = kv_heads;
   p.group = heads / kv_heads;
   p.pair_heads = p.group % 2 == 0;
-  p.causal = causal != 0;
+  p.causal = (flags & QI_B200_ATTN_CAUSAL) != 0;
+  p.zero_rest = zero_rest;
   p.scale_log2e = scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.ldo = ldo;

@@ -276,10 +276,12 @@ inline at::Tensor attention_packed(const at::Tensor& q, const at::Tensor& k, con
        "qi_b200_attention_packed_workspace_bytes");
   at::Tensor ws;
   if (ws_bytes) ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+  // a new output has no contents that its rows outside every sequence could keep
+  const int flags = (causal ? QI_B200_ATTN_CAUSAL : 0) | (given(out) ? 0 : QI_B200_ATTN_ZERO_REST);
   done(qi_b200_attention_packed(ptr(q), ldq, ptr(k), ldk, ptr(v), ldv, ptr(o), ldo, static_cast<float*>(ptr(lse)),
                                 cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), n_seq, static_cast<int>(Tq),
                                 static_cast<int>(Tk), static_cast<int>(heads), static_cast<int>(kv_heads),
-                                static_cast<int>(D), causal, f, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
+                                static_cast<int>(D), flags, f, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
                                 at::cuda::getCurrentCUDAStream(same.dev.index())),
        "qi_b200_attention_packed");
   return o;

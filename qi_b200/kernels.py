@@ -678,8 +678,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     (int32 [n + 1]).  ``causal``: query i sees the keys j <= i + (lk - lq), so
     the last query sees every key; a query that sees none gives zeros.  Query
     head h reads key head h // (heads // kv_heads).  Returns [Tq, heads * D]
-    bf16 (or writes ``out``, which must not overlap the inputs; its rows
-    outside every sequence stay as they were).  ``lse`` fp32 [Tq, heads] receives the log of the softmax sums.
+    bf16, zeros in rows outside every sequence (or writes ``out``, which must
+    not overlap the inputs; there such rows stay as they were).  ``lse`` fp32 [Tq, heads] receives the log of the softmax sums.
     Default scale 1 / sqrt(D)."""
     op = _ops().attention_packed
     if out is None:

@@ -375,3 +375,14 @@ def test_schemas_say_what_is_written_and_returned(name):
     returned = [next(n for n, b in sets.items() if b == r.alias_info.before_set) for r in whole.returns]
     assert returned == {"rms_norm_quant": ["q", "s"], "rope_axes": ["out_q", "out_k"], "rope_axes_store": ["out_q"],
                         "attention_packed": ["out"], "attention_paged": ["out"]}[name]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: for machines without a device")
+def test_c_abi_flags_of_packed_attention():
+    """Flags other than the two are refused; without sequences there is work only where rows are to become zeros."""
+    call = lambda flags, n=1, out=0x1000: _lib.load().qi_b200_attention_packed(
+        0x1000, 256, 0x1000, 128, 0x1000, 128, out, 256, None, 0x1000, 0x1000, n, 4, 4, 2, 1, 128, flags, 1.0, None, 0, None)
+    assert call(4) == call(-1) == _lib.EINVAL
+    assert call(0, n=0) == call(1, n=0, out=None) == _lib.OK
+    assert call(3, n=0, out=None) == call(2, out=None) == _lib.EINVAL
+    assert call(2, n=0) == call(3) == _lib.ECUDA  # the device is asked for

@@ -566,6 +566,32 @@ def test_attention_packed_queries_without_a_key_give_zeros(ql, kl, hq, hk, D):
     close_lse(lse[~hit], wl[~hit])
 
 
+@pytest.mark.parametrize("ql,front,back,hq,hk,D", [
+    ([50, 70], 0, 9, 4, 2, 128), ([300], 5, 0, 3, 3, 64), ([129], 700, 900, 2, 1, 128), ([1500, 0, 40], 1, 3, 4, 4, 64),
+    ([], 0, 33, 2, 2, 128),
+])
+def test_attention_packed_rows_outside_of_a_new_output_are_zeros(ql, front, back, hq, hk, D):
+    """A padded batch: rows that belong to no sequence are zeros in an output that the call allocates, whatever its
+    memory held, and stay as they were in a given one and in lse."""
+    g = gen(sum(ql) + front + hq)
+    n = sum(ql)
+    q, k, v = (randn(g, front + n + back, h * D) for h in (hq, hk, hk))
+    for t in (q, k, v):
+        t[:front], t[front + n:] = float("nan"), float("nan")
+    c = (cu(ql) + front).to(torch.int32)
+    given, lse = torch.full_like(q, 4), torch.full((q.shape[0], hq), 4.0, device=DEV)
+    K.attention_packed(q, k, v, c, c, hq, hk, out=given, lse=lse)
+    used = torch.full_like(q, float("nan"))  # its memory is the next output's
+    at = used.data_ptr()
+    del used
+    o = K.attention_packed(q, k, v, c, c, hq, hk)
+    assert o.data_ptr() == at
+    rest = torch.ones(q.shape[0], dtype=torch.bool, device=DEV)
+    rest[front:front + n] = False
+    assert (o[rest] == 0).all() and (given[rest] == 4).all() and (lse[rest] == 4).all()
+    assert torch.equal(o[~rest], given[~rest]) and torch.isfinite(o).all()
+
+
 def test_attention_packed_nothing_to_do():
     q = torch.zeros(0, 128, dtype=BF, device=DEV)
     assert K.attention_packed(q, q, q, cu([]), cu([]), 1, 1).shape == (0, 128)
