@@ -338,7 +338,8 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
  * pages are page_table[b, :] (int32, device, row stride ld_table, max_pages
  * columns).  A length of 0 gives zeros (lse -inf).  A page outside the cache
  * or a length behind the table reads nothing: those keys take no part, and
- * the device status word is set (code 2).  out must not overlap the inputs.
+ * the device status word is set (code 2); a negative length counts as 0 and
+ * sets it too.  out must not overlap the inputs.
  * The workspace holds partial
  * results of sequences that several SMs share; it needs no initialization and
  * may be used again by the next call on the stream. */

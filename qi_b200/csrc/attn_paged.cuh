@@ -42,7 +42,8 @@
 // nats), and no probability is off by more than 2^-40.
 //
 // A page index outside the cache, or a length behind the page table, reads
-// nothing: those keys take no part, and the device status word is set.
+// nothing: those keys take no part, and the device status word is set.  So it is
+// for a negative length, which counts as 0.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -95,7 +96,8 @@ __device__ __forceinline__ int paged_length(const PagedParams& p, int b) {
     record_error(kDevBadIndex, kTagPaged, 1);
     return static_cast<int>(most);
   }
-  return n < 0 ? 0 : n;
+  if (n < 0) record_error(kDevBadIndex, kTagPaged, 3);
+  return max(n, 0);
 }
 // Tokens per unit: 2^unit_shift.
 __device__ __forceinline__ int paged_units(const PagedParams& p, int len) {

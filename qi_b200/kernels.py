@@ -700,7 +700,7 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     sequence in order; ``lengths`` int32 [B]: its tokens, the new one
     included.  A length of 0 gives zeros.  Entries of ``pages`` behind a
     sequence's last page are not read; a page outside the cache, or a length
-    behind the table, is left out and reported by
+    that is negative or behind the table, is left out and reported by
     ``_lib.raise_on_device_error``.  Returns [B, heads * D] bf16 (or writes
     ``out``, which must not overlap the inputs); ``lse`` fp32 [B, heads] receives the log of the softmax sums."""
     op = _ops().attention_paged

@@ -841,6 +841,20 @@ def test_attention_paged_bad_pages_and_lengths_are_left_out():
     _lib.raise_on_device_error()
 
 
+def test_attention_paged_negative_lengths_are_reported():
+    g = gen(8)
+    table, kc, vc, _ = make_cache(g, [40, 40, 40], 16, 1, 64, "bf16", "token")
+    q = randn(g, 3, 2 * 64)
+    lse = torch.full((3, 2), 3.0, device=DEV)
+    lengths = lambda *n: torch.tensor(n, dtype=torch.int32, device=DEV)
+    o = K.attention_paged(q, kc, vc, table, lengths(40, -1, -(1 << 31)), lse=lse)
+    with pytest.raises(_lib.QiB200DeviceError, match="out of range"):
+        _lib.raise_on_device_error()
+    assert (o[1:] == 0).all() and (lse[1:] == -math.inf).all()
+    assert torch.equal(o, K.attention_paged(q, kc, vc, table, lengths(40, 0, 0)))
+    _lib.raise_on_device_error()
+
+
 # ---------------------------------------------------------------------------
 # streams, graphs, refusals, and all of them together
 # ---------------------------------------------------------------------------
