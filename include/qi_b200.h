@@ -310,7 +310,7 @@ int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk
 
 /* Attention over packed sequences: rows cu_q[b] .. cu_q[b+1] of q attend the
  * rows cu_k[b] .. cu_k[b+1] of k and v (cu_* int32 [n_seq + 1], device,
- * ascending); with ATTN_CAUSAL, query i of a sequence sees the keys
+ * ascending; scale positive, and scale log2(e) finite); with ATTN_CAUSAL, query i of a sequence sees the keys
  * j <= i + (lk - lq).  A query that sees no key gives zeros.  Query head h
  * reads key head h / (heads / kv_heads).  head_dim 64 or 128.  flags: a sum of
  * QI_B200_ATTN_CAUSAL and QI_B200_ATTN_ZERO_REST.  bf16 in and

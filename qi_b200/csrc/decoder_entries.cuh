@@ -15,6 +15,10 @@ namespace qib {
 
 static inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
+// The kernels take powers of two: scale log2(e) has to be finite as well.
+constexpr float kLog2e = 1.4426950408889634f;
+static inline bool softmax_scale_ok(float scale) { return scale > 0.0f && scale * kLog2e <= FLT_MAX; }
+
 // Dynamic shared memory above 48 KB, once per kernel and device.
 template <auto KERNEL>
 static int allow_smem(int bytes) {
@@ -272,7 +276,7 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
   if (static_cast<long long>(total_q) + total_k > 0x3fffffff) return QI_B200_ETOOBIG;  // key places in 32 bits
   if (q == nullptr || out == nullptr || cu_q == nullptr || cu_k == nullptr || (total_k > 0 && (!k || !v)))
     return QI_B200_EINVAL;
-  if (!(scale > 0.0f) || scale > FLT_MAX) return QI_B200_EINVAL;
+  if (!softmax_scale_ok(scale)) return QI_B200_EINVAL;
   const long long wq = static_cast<long long>(heads) * head_dim, wk = static_cast<long long>(kv_heads) * head_dim;
   if (ldq < wq || ldo < wq || ldq % 8 || ldo % 8) return QI_B200_ESHAPE;
   if (total_k > 0 && (ldk < wk || ldv < wk || ldk % 8 || ldv % 8)) return QI_B200_ESHAPE;
@@ -296,7 +300,7 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
   p.pair_heads = p.group % 2 == 0;
   p.causal = (flags & QI_B200_ATTN_CAUSAL) != 0;
   p.zero_rest = zero_rest;
-  p.scale_log2e = scale * 1.4426950408889634f;
+  p.scale_log2e = scale * kLog2e;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.ldo = ldo;
   p.lse = lse;
@@ -344,7 +348,7 @@ int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_ca
   if (q == nullptr || out == nullptr || lengths == nullptr || cache == nullptr || (max_pages > 0 && !page_table) ||
       workspace == nullptr)
     return QI_B200_EINVAL;
-  if (!(scale > 0.0f) || scale > FLT_MAX) return QI_B200_EINVAL;
+  if (!softmax_scale_ok(scale)) return QI_B200_EINVAL;
   const long long wq = static_cast<long long>(heads) * head_dim;
   if (ldq < wq || ldo < wq || ldq % 8 || ldo % 8) return QI_B200_ESHAPE;
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace)) return QI_B200_EALIGN;
@@ -386,7 +390,7 @@ int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_ca
     if (cache->page_size == 1 << s) p.page_shift = s;
   p.max_pages = max_pages;
   p.num_pages = cache->pages;
-  p.scale_log2e = scale * 1.4426950408889634f;
+  p.scale_log2e = scale * kLog2e;
   const int G = di->num_sms;
   // key heads per item: as many as lie next to each other (see the kernel), as
   // long as the longest the lengths may be still gives every SM four units

@@ -245,7 +245,8 @@ inline float softmax_scale(int64_t head_dim, int64_t heads, int64_t kv_heads, co
   if (given(lse)) dense(*lse, "lse", at::kFloat, {rows, heads});
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(head_dim));
   const float f = static_cast<float>(s);
-  TORCH_CHECK_VALUE(f > 0.f && std::isfinite(f), "scale must be positive and finite, got ", s, ".");
+  TORCH_CHECK_VALUE(f > 0.f && std::isfinite(f * 1.4426950408889634f),
+                    "scale must be positive, and finite times log2(e), got ", s, ".");
   return f;
 }
 

@@ -386,3 +386,27 @@ def test_c_abi_flags_of_packed_attention():
     assert call(0, n=0) == call(1, n=0, out=None) == _lib.OK
     assert call(3, n=0, out=None) == call(2, out=None) == _lib.EINVAL
     assert call(2, n=0) == call(3) == _lib.ECUDA  # the device is asked for
+
+
+def test_scales_that_overflow_in_powers_of_two():
+    """A finite scale whose product with log2(e) is not: it would make every score of zero a NaN."""
+    edge = 3.4028234e38 / 1.4426950408889634
+    for call in (packed, paged):
+        for scale in (edge * 1.00001, 3.4e38):
+            with pytest.raises(ValueError, match="scale must be"):
+                call(scale=scale)
+        with pytest.raises(ValueError, match="CUDA tensor"):
+            call(scale=edge * 0.99999)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: for machines without a device")
+def test_c_abi_scales_that_overflow_in_powers_of_two():
+    lib, p = _lib.load(), 0x1000
+    c = _lib.PagedCache(k=p, v=p, pages=4, page_size=16)
+    for field in (c.page_stride, c.slot_stride, c.head_stride):
+        field[:] = (128, 128)
+    for scale, status in ((2.4e38, _lib.EINVAL), (2.3e38, _lib.ECUDA)):  # log2(e) 2.36e38 is the largest number
+        assert lib.qi_b200_attention_packed(p, 256, p, 128, p, 128, p, 256, None, p, p, 1, 4, 4, 2, 1, 128, 1, scale,
+                                            None, 0, None) == status
+        assert lib.qi_b200_attention_paged(p, 256, ctypes.byref(c), p, 4, 4, p, p, 256, None, 2, 2, 1, 128, scale, p,
+                                           1 << 30, None) == status
