@@ -141,6 +141,40 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       : "memory");
 }
 
+// What the roles of a CTA tell each other: one gave up; warps that look at rows
+// once more (packed_mend).
+struct PackedFlags {
+  int abort, mending;
+};
+
+// The softmax warps' wait: mbar_wait_hot, but the limit does not run while a warp
+// is in packed_mend, which ends by itself and takes time by the length of the
+// sequence (32 rows over 300,000 keys take longer than the limit).
+__device__ __forceinline__ bool packed_wait(uint64_t* bar, uint32_t parity, volatile PackedFlags* flags,
+                                            unsigned int tag, unsigned int site) {
+#pragma unroll 1
+  for (int i = 0; i < 512; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = globaltimer_ns();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (flags->abort) return false;
+    if (flags->mending) {
+      t0 = globaltimer_ns();
+    } else if (globaltimer_ns() - t0 > QI_WAIT_TIMEOUT_NS) {
+      record_error(kDevWaitTimeout, tag, site);
+      flags->abort = 1;
+      return false;
+    }
+  }
+}
+// The other roles only have to outlast it: where the pipeline stalls the softmax
+// warps wait too, and give up for the CTA after the usual limit.  (With the
+// check in their waits as well, chunks after prefixes at D = 64 took 2 % longer.)
+constexpr unsigned long long kPackedRoleLimit = 600000000000ull;  // 600 s: a mend over 80 million keys
+
 template <int D>
 struct PackedCfg {
   static constexpr int TILE = 128 * D * 2;       // bytes of a 128-row operand tile (D / 64 swizzled blocks)
@@ -522,7 +556,8 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   uint64_t* it_empty = it_full + kPackedItems;                                 // [kPackedItems]
   PackedItem* items = reinterpret_cast<PackedItem*>(it_empty + kPackedItems);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kPackedItems);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile PackedFlags* flags = reinterpret_cast<volatile PackedFlags*>(tmem_slot + 1);
+  volatile int* abort_flag = &flags->abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -542,7 +577,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       mbar_init(&it_full[i], 1);
       mbar_init(&it_empty[i], 10);  // the softmax warps, TMA and MMA
     }
-    *abort_flag = 0;
+    flags->abort = flags->mending = 0;
     fence_mbar_init();
     tma_prefetch_map(&tmQ);
     tma_prefetch_map(&tmK);
@@ -562,7 +597,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   // the next item (nullptr: none, or the CTA gives up), and its release
   uint32_t n_it = 0;
   auto next_item = [&]() -> const PackedItem* {
-    if (!mbar_wait_hot(&it_full[n_it % kPackedItems], (n_it / kPackedItems) & 1u, abort_flag, kTagPacked, 11))
+    if (!packed_wait(&it_full[n_it % kPackedItems], (n_it / kPackedItems) & 1u, flags, kTagPacked, 11))
       return nullptr;
     const PackedItem* it = &items[n_it % kPackedItems];
     return it->last ? nullptr : it;
@@ -579,7 +614,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       // ---- items ----
       packed_schedule<D>(p, [&](const PackedItem& it) {
         const int i = n_it % kPackedItems;
-        if (!mbar_wait_hot(&it_empty[i], ((n_it / kPackedItems) & 1u) ^ 1u, abort_flag, kTagPacked, 12)) return false;
+        if (!mbar_wait_hot<kPackedRoleLimit>(&it_empty[i], ((n_it / kPackedItems) & 1u) ^ 1u, abort_flag, kTagPacked, 12)) return false;
         if (lane == 0) {
           items[i] = it;
           mbar_arrive(&it_full[i]);
@@ -605,7 +640,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       bool ok = true;
       int q_pend[2] = {0, 0};  // Q loads issued
       auto load = [&](const CUtensorMap* map, int col, int row) {
-        ok = ok && mbar_wait_hot(&kv_empty[stage], (use & 1u) ^ 1u, abort_flag, kTagPacked, 21);
+        ok = ok && mbar_wait_hot<kPackedRoleLimit>(&kv_empty[stage], (use & 1u) ^ 1u, abort_flag, kTagPacked, 21);
         if (!ok) return;
         if (lane == 0) {
           mbar_expect_tx(&kv_full[stage], C::TILE);
@@ -628,7 +663,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (it->n[t] == 0 || !ok) continue;
-            ok = mbar_wait_hot(&q_empty[t], (q_pend[t] & 1) ^ 1, abort_flag, kTagPacked, 22);
+            ok = mbar_wait_hot<kPackedRoleLimit>(&q_empty[t], (q_pend[t] & 1) ^ 1, abort_flag, kTagPacked, 22);
             if (ok && lane == 0) {
               mbar_expect_tx(&q_full[t], C::TILE);
 #pragma unroll
@@ -670,7 +705,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       int valid = 0;                      // keys of the step before that lie inside the sequence
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-        return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag, kTagPacked, site)) != 0;
+        return __all_sync(0xffffffffu, mbar_wait_hot<kPackedRoleLimit>(bar, parity, abort_flag, kTagPacked, site)) != 0;
       };
       auto full = [&](int i, int site) {
         return wait(&kv_full[i % C::STAGES], static_cast<uint32_t>(i / C::STAGES) & 1u, site);
@@ -788,7 +823,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       float m_use = -INFINITY;
       float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       for (int j = steps - 1; j >= 0; --j) {
-        ok = mbar_wait_hot(&s_full[t], n_s & 1u, abort_flag, kTagPacked, 41);
+        ok = packed_wait(&s_full[t], n_s & 1u, flags, kTagPacked, 41);
         if (!ok) break;
         tc_fence_after();
         uint32_t r[4][32];
@@ -866,7 +901,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         part[0] = m_use;
         part[128] = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
         if (steps > 0) {
-          ok = mbar_wait_hot(&o_done[t], n_items++ & 1u, abort_flag, kTagPacked, 44);
+          ok = packed_wait(&o_done[t], n_items++ & 1u, flags, kTagPacked, 44);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -885,7 +920,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       float inv = 0.f;  // a row that saw no key gives zeros
       bool finite = false;
       if (steps > 0) {
-        ok = mbar_wait_hot(&o_done[t], n_items++ & 1u, abort_flag, kTagPacked, 43);
+        ok = packed_wait(&o_done[t], n_items++ & 1u, flags, kTagPacked, 43);
         if (!ok) break;
         tc_fence_after();
         const float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
@@ -961,8 +996,11 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       }
       if (__any_sync(0xffffffffu, bad)) {
         const int col = head / p.group * D;
+        int* mending = const_cast<int*>(&flags->mending);
+        if (lane == 0) atomicAdd(mending, 1);
         packed_mend<D>(bad, limit, end, p.q + (first + lane) * p.ldq + head * D, p.k + it->k0 * p.ldk + col, p.ldk,
                        p.v + it->k0 * p.ldv + col, p.ldv, dst + lane * p.ldo, p.scale_log2e, m_use, inv, -1);
+        if (lane == 0) atomicSub(mending, 1);
       }
       release_item();
     }

@@ -109,6 +109,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // Bounded wait for the phase with the given parity to complete.  Returns
 // false when the CTA is aborting (flag already raised by another role) or
 // when this wait ran out of time (then it raises the flag itself).
+template <unsigned long long LIMIT_NS = QI_WAIT_TIMEOUT_NS>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                           unsigned int tag, unsigned int site) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -118,7 +119,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     for (int i = 0; i < 32; ++i)
       if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
-    if (globaltimer_ns() - t0 > QI_WAIT_TIMEOUT_NS) {
+    if (globaltimer_ns() - t0 > LIMIT_NS) {
       record_error(kDevWaitTimeout, tag, site);
       *abort_flag = 1;
       return false;
@@ -129,12 +130,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 // mbar_wait for handovers on a kernel's critical path: it looks at the timer
 // and the abort flag only after many tries, because reading %globaltimer takes
 // long enough to delay the handover.
+template <unsigned long long LIMIT_NS = QI_WAIT_TIMEOUT_NS>
 __device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                               unsigned int tag, unsigned int site) {
 #pragma unroll 1
   for (int i = 0; i < 512; ++i)
     if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, abort_flag, tag, site);
+  return mbar_wait<LIMIT_NS>(bar, parity, abort_flag, tag, site);
 }
 
 // Wait used only while draining after an abort: shorter limit, no new error.

@@ -592,6 +592,35 @@ def test_attention_packed_rows_outside_of_a_new_output_are_zeros(ql, front, back
     assert torch.equal(o[~rest], given[~rest]) and torch.isfinite(o).all()
 
 
+def test_attention_packed_looks_at_rows_again_for_longer_than_its_waits():
+    """Rows whose outputs are computed once more (a value behind them holds a NaN) over a sequence so long that this
+    takes longer than a wait may: the waits of the CTA's next item do not give up.  Without a workspace nothing is cut,
+    so two items come one after the other."""
+    g = gen(31)
+    hq, D, lq, lk = 300, 64, 129, 400_000
+    q, k, v = randn(g, lq, hq * D), randn(g, lk, D), randn(g, lk, D)
+    v[lk - 60] = float("nan")  # queries 0 to 68 do not see it
+    o = torch.empty_like(q)
+    c, ck = cu([lq]), cu([lk])
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    _lib.check("qi_b200_attention_packed", _lib.load().qi_b200_attention_packed(
+        q.data_ptr(), hq * D, k.data_ptr(), D, v.data_ptr(), D, o.data_ptr(), hq * D, None, c.data_ptr(), ck.data_ptr(), 1,
+        lq, lk, hq, 1, D, 1, 0.5, None, 0, torch.cuda.current_stream().cuda_stream))
+    end.record()
+    torch.cuda.synchronize()
+    _lib.raise_on_device_error()
+    assert start.elapsed_time(end) > 2000  # the limit of a wait: else the test does not show what it is for
+    v[lk - 60] = 0
+    assert torch.isfinite(o[:69]).all() and torch.isnan(o[69:]).all()
+    for h in (0, 148, 299):
+        want, tol, _ = attend_ref(q[:69, h * D:(h + 1) * D], k[:lk - 60], v[:lk - 60], lk - lq, 0.5, 2.0 ** -8)
+        # fp32 sums of 100,000 terms to a chain, each addition off by 2^-24 of the sum so far: 0.006 of sum p|v| and
+        # of the sum of p at worst; tol holds at least 2^-8 sum p|v|, so the first is below 1.6 tol
+        tol = 2.6 * tol + 0.006 * want.abs()
+        assert ((o[:69, h * D:(h + 1) * D].double() - want).abs() <= tol).all()
+
+
 def test_attention_packed_nothing_to_do():
     q = torch.zeros(0, 128, dtype=BF, device=DEV)
     assert K.attention_packed(q, q, q, cu([]), cu([]), 1, 1).shape == (0, 128)
