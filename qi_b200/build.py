@@ -20,7 +20,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libqi_b200.so"
 
 SOURCES = [CSRC / "qi_b200.cu"]
-DEPS = sorted(CSRC.glob("*.cu*")) + [ROOT / "include" / "qi_b200.h"]
+DEPS = sorted(CSRC.glob("*.cu*")) + [CSRC / "attn_split.h", ROOT / "include" / "qi_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -65,6 +65,7 @@
 #include <type_traits>
 
 #include "attn_short.cuh"
+#include "attn_split.h"
 #include "launch_count.cuh"
 #include "sm100_ptx.cuh"
 
@@ -72,13 +73,11 @@ namespace qib {
 
 constexpr unsigned int kTagPacked = 0x900u;
 
-struct PackedParams {
+struct PackedParams : PackedShape {
   const int* cu_q;   // [n_seq + 1]
   const int* cu_k;
   int n_seq, total_q, total_k;
-  int heads, kv_heads, group;
-  int pair_heads;    // 1: an item is two heads x 128 tokens, 0: one head x 256 tokens
-  int causal;
+  int kv_heads, group;
   int zero_rest;     // 1: rows of out outside every sequence become zeros
   float scale_log2e;
   __nv_bfloat16* out;
@@ -171,17 +170,6 @@ struct PackedCfg {
   static constexpr uint32_t IDESC_O = make_idesc(kDF32, kFmtBF16, kFmtBF16, 128, D) | (1u << 16);  // B is MN-major
 };
 
-// One work item, or the part of one that falls to a CTA, as the scheduling
-// warp puts it into shared memory.
-struct PackedItem {
-  int q0, lq;          // first query row and length of the sequence
-  int k0, lk;          // first key row of the part; keys of the sequence from there on
-  int m[2], head[2];   // first token (inside the sequence) and head of the two tiles
-  int n[2];            // 128-key steps of the two tiles (0: nothing visible, or no rows)
-  int diag;            // last visible key of token i is i + diag (counted from k0), at most lk - 1
-  int part;            // -1: whole; else the CTA's workspace place that takes the partial result
-  int last;            // 1: there is no item, the CTA is done
-};
 constexpr int kPackedItems = 4;  // items in flight
 
 // Rows of sequence b, clamped to the tensor (bad prefix sums read and write inside it).
@@ -190,10 +178,6 @@ __device__ __forceinline__ void packed_span(const int* cu, int b, int total, int
   len = min(max(cu[b + 1], first), total) - first;
 }
 
-// First rows and lengths of a sequence (zeros behind the last one).
-struct PackedSpan {
-  int q0, lq, k0, lk;
-};
 __device__ __forceinline__ PackedSpan packed_load(const PackedParams& p, int b) {
   PackedSpan s = {0, 0, 0, 0};
   if (b < p.n_seq) {
@@ -206,47 +190,10 @@ __device__ __forceinline__ PackedSpan packed_from_lane(const PackedSpan& s, int 
   return {__shfl_sync(0xffffffffu, s.q0, lane), __shfl_sync(0xffffffffu, s.lq, lane),
           __shfl_sync(0xffffffffu, s.k0, lane), __shfl_sync(0xffffffffu, s.lk, lane)};
 }
-// 128-key steps of tile t of query block `level`.
-__device__ __forceinline__ int packed_tile_steps(const PackedParams& p, const PackedSpan& s, int level, int t) {
-  const int m = p.pair_heads ? level * 128 : level * 256 + 128 * t;
-  const int rows = min(128, s.lq - m);
-  const int visible = p.causal ? min(s.lk, m + rows + s.lk - s.lq) : s.lk;
-  return rows > 0 && visible > 0 ? (visible + 127) / 128 : 0;
-}
-__device__ __forceinline__ int packed_steps(const PackedParams& p, const PackedSpan& s, int level) {
-  return max(packed_tile_steps(p, s, level, 0), packed_tile_steps(p, s, level, 1));
-}
-
-// Steps [lo, hi) of an item (counted from its first key); whole where that is all of it.
-__device__ __forceinline__ PackedItem packed_item(const PackedParams& p, const PackedSpan& s, int level, int hi_,
-                                                  int lo, int hi, int part) {
-  PackedItem it;
-  it.q0 = s.q0, it.lq = s.lq;
-  it.k0 = s.k0 + lo * 128, it.lk = s.lk - lo * 128;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    it.head[t] = p.pair_heads ? 2 * hi_ + t : hi_;
-    it.m[t] = p.pair_heads ? level * 128 : level * 256 + 128 * t;
-    it.n[t] = max(0, min(packed_tile_steps(p, s, level, t), hi) - lo);
-  }
-  it.diag = p.causal ? it.lk - it.lq : 0x3fffffff - s.lq;
-  it.part = part;
-  it.last = 0;
-  return it;
-}
-
 // One partial result in the workspace: per tile 128 maxima, 128 sums and D
 // columns of 128 fp32 output elements.
 template <int D>
 __host__ __device__ constexpr int packed_part_floats() { return 2 * 128 * (D + 2); }
-// Which item a partial result belongs to; two places per CTA: 0 for an item
-// that an earlier CTA begins, 1 for one that the CTA begins and a later one goes on with.
-struct PackedRecord {
-  int used, ends;           // there is a partial result; it is the item's last
-  int row[2], rows[2], head[2];
-  int k0, end[2], limit[2];  // the item's first key row; keys in its steps; last visible key of the first row
-};
-
 // The rows of a warp (a lane each) once more whose sum is finite and whose
 // output holds a NaN (`bad`), where a key behind the row's last visible one
 // (`limit`) and inside the steps that were multiplied (`end`) has a value that
@@ -335,34 +282,15 @@ __device__ __noinline__ void packed_mend(bool bad, int limit, int end, const __n
   __syncwarp();
 }
 
-// What an item costs beside its steps, in steps (measured: 4 us for an item of
-// one step, 1.8 us for every further one).
-constexpr int kPackedItemCost = 2;
-
-// An even split pays where the longest-first order leaves SMs idle for longer
-// than writing and joining the partial results takes (about 12 us, 7 steps).
-// What that order leaves idle: at most one item per CTA, the longest; equal
-// items, what the last round lacks; falling lengths, about half the length of
-// the last round's items.
-__device__ __forceinline__ bool packed_even_split(long long cost, long long items, int longest, int G, int causal) {
-  const long long even = cost / G;
-  long long order;
-  if (items <= G) order = longest;
-  else if (!causal) order = (items + G - 1) / G * longest;
-  else order = even + static_cast<long long>(longest) * G / (2 * items);
-  return order - even > 7;
-}
-
 // The items of this CTA one after another to `put` (the whole warp calls it).
 // A lane holds the span of a sequence, 32 sequences at a time.
 template <int D, class Put>
 __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) {
   const int lane = threadIdx.x & 31;
-  const int block_shift = p.pair_heads ? 7 : 8;  // query rows per item
-  const int heads_items = p.pair_heads ? p.heads / 2 : p.heads;
+  const int heads_items = packed_head_items(p);
   const int G = gridDim.x, me = blockIdx.x;
   PackedSpan span = packed_load(p, lane);
-  auto blocks = [&](const PackedSpan& s) { return (s.lq + (1 << block_shift) - 1) >> block_shift; };
+  auto blocks = [&](const PackedSpan& s) { return packed_blocks(p, s); };
   auto end_of_items = [&]() {
     PackedItem end = {};
     end.last = 1;
@@ -371,23 +299,13 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
   int most = 0, longest = 0, count = 0;
   int chunk_most = 0;  // most blocks of a sequence in the lane's chunk of 32 (of the first 32 chunks)
   long long total = 0;
-  auto seq_cost = [&](const PackedSpan& s) {  // cost of one head item of each block with keys
-    const int nb = blocks(s);
-    int sum = 0;
-    for (int level = 0; level < nb; ++level) {
-      const int n = packed_steps(p, s, level);
-      sum += n + (n > 0 ? kPackedItemCost : 0);
-      longest = max(longest, n + kPackedItemCost);
-    }
-    return sum;
-  };
   for (int chunk = 0; chunk < p.n_seq; chunk += 32) {
     const PackedSpan s = chunk ? packed_load(p, chunk + lane) : span;
     const int chunk_max = __reduce_max_sync(0xffffffffu, blocks(s));
     most = max(most, chunk_max);
     if (lane == chunk >> 5) chunk_most = chunk_max;
     if (p.ws != nullptr) {
-      total += seq_cost(s);
+      total += packed_seq_cost(p, s, longest);
       count += blocks(s);
     }
   }
@@ -403,13 +321,8 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
     }
     total *= heads_items;
     if (packed_even_split(total, static_cast<long long>(count) * heads_items, longest, G, p.causal)) {
-      // the costs of all items end to end (sequences in order, blocks in order,
-      // heads; an item's fixed cost, then its steps from the last to the first),
-      // cut into equal ranges long enough for three steps, so that the parts of an
-      // item are those of consecutive CTAs
-      const long long cuts = max(1ll, min(static_cast<long long>(G), total / (kPackedItemCost + 3)));
-      const long long lo = total * min(static_cast<long long>(me), cuts) / cuts;
-      const long long hi = total * min(me + 1ll, cuts) / cuts;
+      const long long cuts = packed_cuts(total, G);
+      const long long lo = packed_cut_begin(total, cuts, me), hi = packed_cut_begin(total, cuts, me + 1);
       auto scan = [&](long long v) {  // inclusive, over the lanes
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -418,12 +331,12 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
         }
         return v;
       };
-      auto cost_of = [&](int steps) { return steps > 0 ? (steps + kPackedItemCost) * static_cast<long long>(heads_items) : 0; };
+      auto cost_of = [&](int steps) { return packed_cost(steps) * static_cast<long long>(heads_items); };
       long long before = 0;  // cost of the sequences in front of the chunk
       int idle = 0;          // blocks without steps so far (zeros to write: the CTAs take turns at them)
       for (int chunk = 0; chunk < p.n_seq; chunk += 32) {
         if (chunk) span = packed_load(p, chunk + lane);
-        const long long mine = static_cast<long long>(seq_cost(span)) * heads_items;
+        const long long mine = packed_seq_cost(p, span, longest) * heads_items;
         const long long end = before + scan(mine);
         unsigned todo = __ballot_sync(0xffffffffu, end > lo && end - mine < hi && mine > 0);
         while (todo) {
@@ -439,30 +352,14 @@ __device__ __forceinline__ void packed_schedule(const PackedParams& p, Put put) 
             while (levels) {
               const int j = __ffs(levels) - 1;
               levels &= levels - 1;
-              const int n = __shfl_sync(0xffffffffu, s_lane, j), per = n + kPackedItemCost;
+              const int n = __shfl_sync(0xffffffffu, s_lane, j), per = packed_cost(n);
               const long long first = __shfl_sync(0xffffffffu, l_end, j) - cost_of(n);
               int h = first < lo ? static_cast<int>((lo - first) / per) : 0;
               for (long long u = first + static_cast<long long>(h) * per; h < heads_items && u < hi; ++h, u += per) {
-                const int from = static_cast<int>(max(0ll, lo - u - kPackedItemCost));
-                const int to = static_cast<int>(max(0ll, min(static_cast<long long>(n), hi - u - kPackedItemCost)));
-                if (from >= to) continue;
-                const int part = from == 0 && to == n ? -1 : (from == 0 ? 1 : 0);
-                const PackedItem it = packed_item(p, s, l0 + j, h, n - to, n - from, part);
-                if (part >= 0 && lane == 0) {
-                  PackedRecord r;
-                  r.used = 1;
-                  r.ends = to == n;
-#pragma unroll
-                  for (int t = 0; t < 2; ++t) {
-                    r.row[t] = it.q0 + it.m[t];
-                    r.rows[t] = max(0, min(128, it.lq - it.m[t]));
-                    r.head[t] = it.head[t];
-                    r.end[t] = min(s.lk, 128 * packed_tile_steps(p, s, l0 + j, t));
-                    r.limit[t] = it.m[t] + it.diag + 128 * (n - to);
-                  }
-                  r.k0 = s.k0;
-                  rec[part] = r;
-                }
+                const PackedCut c = packed_cut_item(u, n, lo, hi);
+                if (c.from >= c.to) continue;
+                const PackedItem it = packed_item(p, s, l0 + j, h, n - c.to, n - c.from, c.part);
+                if (c.part >= 0 && lane == 0) rec[c.part] = packed_record(p, s, l0 + j, n, c.to, it);
                 if (!put(it)) return;
               }
             }

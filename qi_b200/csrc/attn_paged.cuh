@@ -53,6 +53,7 @@
 #include <cstdint>
 
 #include "attn_short.cuh"
+#include "attn_split.h"
 #include "launch_count.cuh"
 #include "sm100_ptx.cuh"
 
@@ -101,7 +102,7 @@ __device__ __forceinline__ int paged_length(const PagedParams& p, int b) {
 }
 // Tokens per unit: 2^unit_shift.
 __device__ __forceinline__ int paged_units(const PagedParams& p, int len) {
-  return static_cast<int>((static_cast<long long>(len) + (1 << p.unit_shift) - 1) >> p.unit_shift);
+  return paged_unit_count(len, p.unit_shift);
 }
 // The item that a CTA begins and later ones go on with, up to CTA `last`.
 struct PagedRecord {
@@ -110,15 +111,6 @@ struct PagedRecord {
 template <int D>
 __device__ __forceinline__ PagedRecord* paged_records(const PagedParams& p, int ctas) {
   return reinterpret_cast<PagedRecord*>(p.ws + ((2ll * ctas) << p.team_shift) * paged_part_floats<D>());
-}
-
-// Ranges that T units are cut into: none of them is empty, so the partial
-// results of an item are those of consecutive CTAs.
-__device__ __forceinline__ long long paged_ranges(long long T, int ctas) { return T < ctas ? T : ctas; }
-
-// CTA whose range [c T / G, (c + 1) T / G) holds unit u.
-__device__ __forceinline__ int paged_owner(long long u, long long T, long long G) {
-  return static_cast<int>(((u + 1) * G - 1) / T);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -248,8 +240,8 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
   }
   if (T == 0) return;
   const long long G = paged_ranges(T, gridDim.x);
-  long long u = T * blockIdx.x / G;
-  const long long u_end = blockIdx.x < G ? T * (blockIdx.x + 1) / G : u;
+  long long u = paged_range_begin(blockIdx.x, T, G);
+  const long long u_end = blockIdx.x < G ? paged_range_begin(blockIdx.x + 1, T, G) : u;
   before += incl - mine;
   if (u < u_end && before <= u && u < before + mine) {
     long long at = before;
