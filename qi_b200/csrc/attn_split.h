@@ -93,7 +93,7 @@ constexpr int kPackedItemCost = 2;
 QIB_SPLIT int packed_cost(int n) { return n > 0 ? n + kPackedItemCost : 0; }
 QIB_SPLIT long long packed_seq_cost(const PackedShape& p, const PackedSpan& s, int& longest) {
   const int nb = packed_blocks(p, s);
-  int sum = 0;
+  long long sum = 0;
   for (int level = 0; level < nb; ++level) {
     const int n = packed_steps(p, s, level);
     sum += packed_cost(n);

@@ -191,6 +191,15 @@ def test_when_packed_items_are_cut(lib, lq, lk, heads, pair, causal, even):
     assert items_of(lib, lq, lk, heads, pair, causal, 148)[0] == even
 
 
+def test_cost_of_long_sequences_passes_32_bits(lib):
+    """2,368 query blocks (16 for each of 148 SMs) over 2^29 keys."""
+    longest = I(0)
+    lq, lk = 2368 * 128, 1 << 29
+    want = sum(-(-(128 * (level + 1) + lk - lq) // 128) + 2 for level in range(2368))
+    assert lib.seq_cost(1, 1, lq, lk, ctypes.byref(longest)) == want > 1 << 32
+    assert longest.value == (1 << 22) + 2
+
+
 @pytest.mark.parametrize("seed", range(20))
 def test_ranges_of_paged_units(lib, seed):
     """The ranges are those of consecutive units, none empty, and the owner of a unit is the CTA whose range holds it;
