@@ -34,7 +34,8 @@
 //
 // E4M3 caches: codes are widened exactly to fp16 and multiplied in fp16 with
 // fp32 sums; q is scaled by a power of two per head so that it fits fp16, the
-// key scale goes into the softmax scale and the value scale into the output.
+// key scale goes into the softmax scale and the value scale into the quotient
+// of output and sum (the sums before it may pass fp32 with it).
 // P is rounded to fp16, whose range ends at 2^-24: what lies far below a row's
 // maximum would be lost, although it makes up the output where the maximum's own
 // value is near zero.  So the base is 2^15 below the maximum and does not lag:
@@ -76,7 +77,7 @@ struct PagedParams {
   long long ldo;
   float* lse;                              // [B, heads] or nullptr
   float* ws;
-  const float* scale[2];                   // E4M3: k_scale, v_scale, [1] or [kv_heads]
+  const float* scale[2];                   // E4M3: k_scale, v_scale, [1] or [kv_heads]; else nullptr
   int scale_per_head[2];
   int B, heads, kv_heads, group, chunks;   // chunks of kPagedRows query heads per key head
   int team_shift, groups;                  // log2 of the key heads per item; kv_heads in such groups
@@ -562,7 +563,6 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
       const int r = i / (D / 2), d = (i - r * (D / 2)) * 2;
       const int of = r / rows, row = r - of * rows;  // key head of the group, query head of its chunk
       const int kv = (kv_group << p.team_shift) + of, head = kv * p.group + chunk * kPagedRows + row;
-      const float v_scale = FP8 ? p.scale[1][p.scale_per_head[1] ? kv : 0] : 1.f;
       float m = -INFINITY;
       for (int w = of; w < W; w += 1 << p.team_shift) m = fmaxf(m, mg_m[w * R + row]);
       const float base = m == -INFINITY ? 0.f : m;
@@ -576,9 +576,10 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
         acc.y = fmaf(v.y, f, acc.y);
       }
       if (whole) {
-        const float inv = l != 0.f ? v_scale / l : 0.f;  // a sum of NaN stays one
+        const float inv = l != 0.f ? 1.f / l : 0.f;  // a sum of NaN stays one
+        const float v_scale = FP8 ? p.scale[1][p.scale_per_head[1] ? kv : 0] : 1.f;
         *reinterpret_cast<__nv_bfloat162*>(p.out + static_cast<long long>(b) * p.ldo + static_cast<long long>(head) * D +
-                                           d) = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+                                           d) = __floats2bfloat162_rn(acc.x * inv * v_scale, acc.y * inv * v_scale);
         if (p.lse != nullptr && d == 0)
           p.lse[static_cast<long long>(b) * p.heads + head] = (m + log2f(l)) * 0.69314718055994531f;
       } else {
@@ -587,7 +588,7 @@ __global__ void __launch_bounds__(PagedCfg<D, FP8>::THREADS, 1) k_attn_paged(con
           part[row] = m;
           part[kPagedRows + row] = l;
         }
-        *reinterpret_cast<float2*>(part + 2 * kPagedRows + row * D + d) = make_float2(acc.x * v_scale, acc.y * v_scale);
+        *reinterpret_cast<float2*>(part + 2 * kPagedRows + row * D + d) = acc;
       }
     }
     __syncthreads();  // the rings are filled again for the next item
@@ -635,7 +636,8 @@ __global__ void __launch_bounds__(kPagedJoinWarps * 32) k_attn_paged_join(const 
 #pragma unroll
   for (int k = 0; k < N; ++k) sm_o[warp][32 * k + lane] = acc[k];
   __syncthreads();
-  const int head = ((r.kv_group << p.team_shift) + of) * p.group + r.chunk * kPagedRows + row;
+  const int kv = (r.kv_group << p.team_shift) + of, head = kv * p.group + r.chunk * kPagedRows + row;
+  const float v_scale = p.scale[1] != nullptr ? p.scale[1][p.scale_per_head[1] ? kv : 0] : 1.f;
   for (int d = threadIdx.x; d < D; d += kPagedJoinWarps * 32) {
     float top = -INFINITY, sum = 0.f, o = 0.f;
 #pragma unroll
@@ -648,7 +650,7 @@ __global__ void __launch_bounds__(kPagedJoinWarps * 32) k_attn_paged_join(const 
       o = fmaf(sm_o[w][d], f, o);
     }
     p.out[static_cast<long long>(r.b) * p.ldo + static_cast<long long>(head) * D + d] =
-        __float2bfloat16_rn(sum != 0.f ? o / sum : 0.f);
+        __float2bfloat16_rn(sum != 0.f ? o / sum * v_scale : 0.f);
     if (p.lse != nullptr && d == 0)
       p.lse[static_cast<long long>(r.b) * p.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
   }

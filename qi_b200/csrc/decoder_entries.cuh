@@ -369,7 +369,7 @@ int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_ca
     p.page_stride[c] = cache->page_stride[c] * elt;
     p.slot_stride[c] = cache->slot_stride[c] * elt;
     p.head_stride[c] = cache->head_stride[c] * elt;
-    p.scale[c] = cache->scale[c];
+    p.scale[c] = cache->fp8 ? cache->scale[c] : nullptr;
     p.scale_per_head[c] = cache->scale_per_head[c];
   }
   p.pages = page_table;

@@ -792,6 +792,22 @@ def test_attention_paged_sinks(kind, lens, hq, hk, D, page, nats, spread):
     close_lse(lse[some], wl)
 
 
+@pytest.mark.parametrize("lens", [[40, 300] * 60, [20000, 33]])
+@pytest.mark.parametrize("v_scale", [1e-37, 1e-20, 1e20, 2e36])
+def test_attention_paged_value_scales_of_many_magnitudes(lens, v_scale):
+    """Items inside one range and items that are cut and joined: outputs lie inside bf16's range, and no sum on the way
+    leaves fp32's."""
+    g = gen(len(lens))
+    table, kc, vc, (ks, _) = make_cache(g, lens, 16, 2, 64, "fp8", "token")
+    vs = torch.tensor([v_scale, v_scale / 3], device=DEV)
+    q = randn(g, len(lens), 4 * 64)
+    o = K.attention_paged(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device=DEV), k_scale=ks, v_scale=vs)
+    some = [0, 1, len(lens) - 1]
+    want, tol, _ = paged_ref(q[some], kc, vc, table[some], [lens[b] for b in some], ks, vs, 64 ** -0.5, "fp8")
+    tol = tol - 1e-30 + 2.0 ** -134  # half a step of bf16's smallest numbers in place of the reference's floor
+    assert ((o[some].double() - want).abs() <= tol).all(), ((o[some].double() - want).abs() / tol).max().item()
+
+
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
 def test_attention_paged_garbage_behind_the_length(kind):
     """Slots behind a sequence's last token hold NaN (bf16 and E4M3 have one): the result does not see them."""
