@@ -310,17 +310,16 @@ int qi_b200_rope_axes(const void* q, long long ldq, const void* k, long long ldk
 
 /* Attention over packed sequences: rows cu_q[b] .. cu_q[b+1] of q attend the
  * rows cu_k[b] .. cu_k[b+1] of k and v (cu_* int32 [n_seq + 1], device,
- * ascending; scale positive, and scale log2(e) finite); with ATTN_CAUSAL, query i of a sequence sees the keys
- * j <= i + (lk - lq).  A query that sees no key gives zeros.  Query head h
+ * ascending; scale positive, and scale log2(e) finite); with ATTN_CAUSAL,
+ * query i of a sequence sees the keys j <= i + (lk - lq).  A query that sees no key gives zeros.  Query head h
  * reads key head h / (heads / kv_heads).  head_dim 64 or 128.  flags: a sum of
- * QI_B200_ATTN_CAUSAL and QI_B200_ATTN_ZERO_REST.  bf16 in and
- * out, fp32 scores and sums, probabilities rounded to bf16 before the product
+ * QI_B200_ATTN_CAUSAL and QI_B200_ATTN_ZERO_REST.  bf16 in and out, fp32 scores and sums, probabilities rounded to bf16 before the product
  * with V.  lse (optional, fp32 [total_q, heads]): log of the sum of
  * exp(scale q.k), -inf where no key is seen.  Rows of out (and lse) outside
  * every sequence are left as they were, but those of out become zeros with
- * QI_B200_ATTN_ZERO_REST.  An infinity or a NaN reaches the
- * queries that see it and no others.  out must not overlap the inputs.  With a workspace of the size that
- * qi_b200_attention_packed_workspace_bytes names (0: none is of use), items
+ * QI_B200_ATTN_ZERO_REST.  An infinity or a NaN reaches the queries that see
+ * it and no others.  out must not overlap the inputs.  With a workspace of the
+ * size that qi_b200_attention_packed_workspace_bytes names (0: none is of use), items
  * may be cut over several SMs where they do not fill the device evenly; it
  * needs no initialization and may be used again by the next call on the
  * stream.  Without one (null, or smaller) nothing is cut. */
@@ -339,9 +338,10 @@ int qi_b200_attention_packed(const void* q, long long ldq, const void* k, long l
  * columns).  A length of 0 gives zeros (lse -inf).  A page outside the cache
  * or a length behind the table reads nothing: those keys take no part, and
  * the device status word is set (code 2); a negative length counts as 0 and
- * sets it too.  out must not overlap the inputs.
- * The workspace holds partial
- * results of sequences that several SMs share; it needs no initialization and
+ * sets it too.  Over an E4M3 cache probabilities are rounded to fp16 above a
+ * base 2^-15 of the row's largest: relative to the largest, one is off by 2^-11
+ * of itself or by 2^-40, whichever is more.  out must not overlap the inputs.
+ * The workspace holds partial results of sequences that several SMs share; it needs no initialization and
  * may be used again by the next call on the stream. */
 int qi_b200_attention_paged_workspace_bytes(int kv_heads, int head_dim, size_t* bytes);
 int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_cache* cache, const int* page_table,

@@ -33,11 +33,15 @@
 // What bounds it: the chain of one tile, softmax (about 2,200 clocks, 1,024 of
 // them exponentials) then P V and S (1,300 clocks, 1,024 of them products),
 // 3,600 clocks per 128-key step where the products of both tiles take 2,048.
-// Measured on the way (16384 tokens, 24 / 8 heads of 128, causal, us; 1,263 is
-// 1,306 TFLOP/s): products issued by lane 0 with 64-bit descriptors formed on
+// At D = 64 the products take half of that and the exponentials as much as before.
+// (TMEM is full at D = 128; at D = 64 columns 384 to 511 are free, and a third S
+// buffer there has not been tried.)
+// Measured on the way (16384 tokens, 24 / 8 heads of 128, causal, us in a short
+// burst; 1,266 is 1,303 TFLOP/s; calls back to back for a second take 1,450 to
+// 1,500 under the 1000 W cap): products issued by lane 0 with 64-bit descriptors formed on
 // the spot 1,842, by an elected thread 1,645, item list in a warp of its own and
 // descriptors as constants to a base 1,371, all MMA operands warp-uniform 1,330,
-// S loaded in one go 1,297, the masked keys in one branch 1,263.  Two threads
+// S loaded in one go 1,297, the masked keys in one branch 1,266.  Two threads
 // per row (16 softmax warps) 1,433; half of P handed over early 1,359; 64-key
 // steps with S double-buffered 1,457 (the products read shared memory at its
 // full rate then, and every barrier waits behind them); a quarter of the

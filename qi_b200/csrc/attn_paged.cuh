@@ -1,8 +1,9 @@
 // Attention of one new token per sequence over a paged key-value cache:
 //   o_b = softmax(scale q_b K_b^T) V_b   per head, grouped heads,
 // K_b, V_b being the first lengths[b] rows that the page table of sequence b
-// names.  Bound: HBM, every cached row is read once and serves all query
-// heads of its key head.
+// names.  Bound: HBM, every cached row is read once for every 16 query heads of
+// its key head (8 sequences of 32768 tokens, one key head of 128, bf16: 37 us with
+// 16 query heads, 46 with 24, 48 with 32).
 //
 // An item is a sequence, a group of 1 to 8 key heads and a chunk of 16 query
 // heads of each.  Where the heads of a cached token lie next to each other, the

@@ -54,8 +54,12 @@ static int check_paged_cache(const qi_b200_paged_cache* c, int kv_heads, int hea
 template <int FMT>
 static int launch_rms_quant(const RmsQuantParams& p, cudaStream_t stream) {
   const int nvec = p.D / 8;
-  // chunks per thread: 4 while that leaves whole warps busy, so that a row's
-  // loads are in flight together; a few rows spread over more threads instead
+  // chunks per thread: 4, so that a row's loads are in flight together; a few rows
+  // spread over more threads instead.  Measured with 1 and 4 (INT8, residual, us):
+  // 200 rows of 1024 / 4096 / 8192 2.4, 3.5, 4.7 against 3.7, 4.1, 4.7; 256 rows
+  // 2.4, 3.5, 6.1 against 3.8, 4.1, 4.8; 777 rows 2.9, 7.4, 10.8 against 3.8, 6.9,
+  // 9.9; 2048 rows 5.0, 15.2, 26.7 against 4.6, 11.2, 25.0 (1024-wide rows alone
+  // would gain from 1 up to 1024 rows)
   const int C = p.M < 256 ? 1 : 4;
   int T = std::min(512, (nvec + 32 * C - 1) / (32 * C) * 32);
   int p2 = 32;
@@ -393,7 +397,11 @@ int qi_b200_attention_paged(const void* q, long long ldq, const qi_b200_paged_ca
   p.scale_log2e = scale * kLog2e;
   const int G = di->num_sms;
   // key heads per item: as many as lie next to each other (see the kernel), as
-  // long as the longest the lengths may be still gives every SM four units
+  // long as the longest the lengths may be still gives every SM four units.  The
+  // host knows the page table's width, not the lengths: with a table much wider
+  // than its sequences a few short ones get items meant for long ones (one
+  // sequence of 1000 tokens, 8 key heads: 8.9 us with a table of 63 pages, 16.6
+  // with 2048; 8 of about 500 tokens 14.5 and 18.8; 64 of them 38.0 and 38.5)
   // a unit holds a whole number of a warp's blocks (16 tokens of 256-byte rows,
   // else 32), so that blocks keep to multiples of their size and to one page
   const int block_shift = head_dim * elt == 256 ? 4 : 5;

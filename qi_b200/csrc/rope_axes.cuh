@@ -21,6 +21,8 @@
 // Measured: 16384 rows of 32 / 8 heads of 128 into an E4M3 cache 70 us (5.3
 // TB/s; 102 us with integer divisions for the places of a unit and unpacked
 // arithmetic), 3120 rows of 24 / 24 heads 16.3 us (4.7 TB/s), 64 rows 2.9 us.
+// Even / odd pairs take 70 to 77 registers, so three CTAs an SM: the 1,560 CTAs of
+// those 3120 rows are 3.5 waves; (i, i + P) pairs take 64, four CTAs.
 // A warp per token: 3120 rows 14 us, but the prompt 74 at best; 128, 192, 384 or
 // 512 threads or 8 tokens a CTA: the prompt no faster.
 // The units whose loads a thread keeps in flight: 2 or 3 the same, 6 slower

@@ -2,8 +2,8 @@
 // use: mbarriers with bounded waits, TMA tiled loads (one destination CTA each),
 // tcgen05 tensor-memory allocation, MMA, commit and loads.
 //
-// Every wait in this file is bounded: after QI_WAIT_TIMEOUT_NS of wall time
-// (read from %globaltimer) it records an error in the device status word,
+// Every wait in this file is bounded: after QI_WAIT_TIMEOUT_NS of wall time (or
+// the limit it is given; read from %globaltimer) it records an error in the device status word,
 // raises the CTA's abort flag and returns false, so a kernel whose pipeline
 // stalls returns an error to the host instead of hanging the GPU.
 #pragma once
