@@ -21,9 +21,8 @@
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of tile 0 and 1, warp 8 TMA,
 // warp 9 MMA, warp 10 the list of items, warp 11 zeros for the rows outside every
-// sequence where they are asked for.  A softmax
-// thread holds a whole row of S, so the softmax warpgroups take 208 registers a
-// thread and the third leaves them all but 88 (of 168 at launch: 256 x 208 +
+// sequence where they are asked for.  A softmax thread holds a whole row of S, so
+// the softmax warpgroups take 208 registers a thread and the third leaves them all but 88 (of 168 at launch: 256 x 208 +
 // 128 x 88 = 64,512, all of them).  CTAs are persistent; each takes every
 // gridDim.x-th item, longest items first, the direction alternating from round
 // to round.  The order is a function of cu_q alone: level L (the L-th query
@@ -38,8 +37,8 @@
 // buffer there has not been tried.)
 // Measured on the way (16384 tokens, 24 / 8 heads of 128, causal, us in a short
 // burst; 1,266 is 1,303 TFLOP/s; calls back to back for a second take 1,450 to
-// 1,500 under the 1000 W cap): products issued by lane 0 with 64-bit descriptors formed on
-// the spot 1,842, by an elected thread 1,645, item list in a warp of its own and
+// 1,500 under the 1000 W cap): products issued by lane 0 with 64-bit descriptors
+// formed on the spot 1,842, by an elected thread 1,645, item list in a warp of its own and
 // descriptors as constants to a base 1,371, all MMA operands warp-uniform 1,330,
 // S loaded in one go 1,297, the masked keys in one branch 1,266.  Two threads
 // per row (16 softmax warps) 1,433; half of P handed over early 1,359; 64-key
@@ -496,7 +495,8 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       // ---- items ----
       packed_schedule<D>(p, [&](const PackedItem& it) {
         const int i = n_it % kPackedItems;
-        if (!mbar_wait_hot<kPackedRoleLimit>(&it_empty[i], ((n_it / kPackedItems) & 1u) ^ 1u, abort_flag, kTagPacked, 12)) return false;
+        if (!mbar_wait_hot<kPackedRoleLimit>(&it_empty[i], ((n_it / kPackedItems) & 1u) ^ 1u, abort_flag, kTagPacked, 12))
+          return false;
         if (lane == 0) {
           items[i] = it;
           mbar_arrive(&it_full[i]);

@@ -29,8 +29,8 @@
 // over the same K and V fragments.  P^T goes from S^T's accumulator layout to
 // the operand layout with one 8 x 8 transpose per 8 tokens.  Powers P = 2^(s - base)
 // are taken above a base that follows the maximum; bf16 caches let it lag by
-// up to 2^8, so most blocks need one vote and no reduction.  The tensor work is a few per cent of what the SM can
-// do, so the legacy instruction is enough; what counts are the bytes in flight
+// up to 2^8, so most blocks need one vote and no reduction.  The tensor work is a
+// few per cent of what the SM can do, so the legacy instruction is enough; what counts are the bytes in flight
 // (128 KB per SM) and the instructions per byte.
 //
 // E4M3 caches: codes are widened exactly to fp16 and multiplied in fp16 with
